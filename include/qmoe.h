@@ -400,6 +400,18 @@ QMOE_API int qmoe_qk_norm_rope(const void* qkv, const int32_t* positions, const 
                                void* q_out, void* k_cache, void* v_cache, int64_t n_slots,
                                int64_t max_seq, void* stream);
 
+/* qmoe_qk_norm_rope with the cache row apart from the position, as a cache
+ * behind a shared prefix and a cache that evicts rows need it: token t's key
+ * and value go to row cache_rows[t] of its slot (NULL: row positions[t]), with
+ * the rotation of positions[t].  row_tokens / row_weights (n_slots, nkv,
+ * max_seq) int32 / fp32, both or neither: the row's entries are set to
+ * positions[t] and 0 for every KV head (qmoe_kv_evict reads them). */
+QMOE_API int qmoe_qk_norm_rope_rows(const void* qkv, const int32_t* positions, const int32_t* cache_rows,
+                                    const int32_t* cache_slot, const float* q_norm_w, const float* k_norm_w,
+                                    const float* inv_freq, int64_t T, int64_t nh, int64_t nkv, int64_t head_dim,
+                                    float eps, void* q_out, void* k_cache, void* v_cache, int32_t* row_tokens,
+                                    float* row_weights, int64_t n_slots, int64_t max_seq, void* stream);
+
 /* ------------------------------------------------------------------------
  * K5  causal GQA flash-prefill over the KV cache (NxDI attention with the
  * flash kernel of qwen.py:25-28, 49).  B sequences of S queries each:
@@ -437,6 +449,92 @@ QMOE_API int qmoe_attention_decode(const void* q, const void* k_cache, const voi
                                    int64_t nh, int64_t nkv, int64_t head_dim, int64_t n_slots,
                                    int64_t max_seq, int64_t max_len, int64_t nsplit, float scale,
                                    void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Attention for a batch that shares a prefix, and attention that keeps every
+ * cache row's weight (no counterpart in the reference).  head_dim 128, any nh
+ * with nh / nkv from 1 to 16, scale positive and finite, statistics in fp32.
+ *
+ * The prefix: rows 0 .. prefix_len-1 of slot prefix_slot of a cache
+ *   k_prefix / v_prefix (n_prefix_slots, nkv, prefix_max, 128) bf16, the same
+ *   for every sequence of the call; its keys carry their own rotations.
+ *   prefix_len 0: none (the pointers may be NULL).  It may be a slot of
+ *   k_cache / v_cache.
+ * Own rows: kv_start[b] .. of slot cache_slot[b] (NULL: slot b), as in
+ *   qmoe_attention_prefill / _decode.  Rows outside the visible ranges, and
+ *   what they hold (NaN and infinities included), reach no output.
+ * weights (n_slots, nkv, max_seq) fp32: weights[slot, g, j] becomes (with
+ *   accumulate: += ) the sum over the KV head's query heads, and over the
+ *   queries, of the attention probability of own row j; without accumulate
+ *   rows of [0, kv_start) become 0; rows at or past the sequence's length are
+ *   left as they were.  A slot given twice in one call: device error 4 and
+ *   only its first entry's weights.
+ * A length, q_start or slot outside its cache or past max_len: device error
+ *   4; the sequence counts as empty (decode) or its rows are not written
+ *   (prefill, weights).
+ *
+ * qmoe_attention_prefix_decode: one query per sequence, q (B, nh, 128) bf16,
+ *   over the prefix and own rows up to kv_len[b] - 1 (kv_len[b] <= max_len;
+ *   0 allowed).  A query that sees no row gets zeros.  weights NULL: none.
+ *   workspace: _workspace_size() bytes, 256-byte aligned, any contents; calls
+ *   that share one must not overlap on the GPU.  Up to 64 rows (B * nh/nkv)
+ *   the prefix streams through warp-level MMA tiles of 16 rows, above that
+ *   through tcgen05 tiles of 128.
+ * qmoe_attention_prefix_prefill: S queries per sequence, q (B*S, nh, 128);
+ *   query i sees the prefix and own rows up to q_start[b] + i.  A query
+ *   before kv_start (a padding position) gets a zero row.  lse (B*S, nh) fp32
+ *   or NULL: natural log-sum-exp of each row's scaled scores, -inf for such.
+ * qmoe_attention_weights: weights of S queries over own rows, from the lse
+ *   of their rows (of qmoe_attention_prefix_prefill; the prefix's share stays
+ *   in it).  max_len bounds q_start + S.
+ * ---------------------------------------------------------------------- */
+QMOE_API int64_t qmoe_attention_prefix_decode_parts(int64_t B, int64_t nh, int64_t nkv, int64_t prefix_len,
+                                                    int64_t max_len);
+QMOE_API size_t qmoe_attention_prefix_decode_workspace_size(int64_t B, int64_t nh, int64_t nkv, int64_t prefix_len,
+                                                            int64_t max_len, int with_weights);
+QMOE_API int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void* v_prefix,
+                                          int64_t n_prefix_slots, int64_t prefix_max, int64_t prefix_slot,
+                                          int64_t prefix_len, const void* k_cache, const void* v_cache,
+                                          const int32_t* kv_len, const int32_t* cache_slot,
+                                          const int32_t* kv_start, int64_t B, int64_t nh, int64_t nkv,
+                                          int64_t head_dim, int64_t n_slots, int64_t max_seq, int64_t max_len,
+                                          float scale, float* weights, int accumulate, void* out, void* workspace,
+                                          size_t workspace_bytes, void* stream);
+QMOE_API int qmoe_attention_prefix_prefill(const void* q, const void* k_prefix, const void* v_prefix,
+                                           int64_t n_prefix_slots, int64_t prefix_max, int64_t prefix_slot,
+                                           int64_t prefix_len, const void* k_cache, const void* v_cache,
+                                           const int32_t* q_start, const int32_t* cache_slot,
+                                           const int32_t* kv_start, int64_t B, int64_t S, int64_t nh, int64_t nkv,
+                                           int64_t head_dim, int64_t n_slots, int64_t max_seq, float scale,
+                                           void* out, float* lse, void* stream);
+QMOE_API int qmoe_attention_weights(const void* q, const float* lse, const void* k_cache, const int32_t* q_start,
+                                    const int32_t* cache_slot, const int32_t* kv_start, int64_t B, int64_t S,
+                                    int64_t nh, int64_t nkv, int64_t head_dim, int64_t n_slots, int64_t max_seq,
+                                    int64_t max_len, float scale, float* weights, int accumulate, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Eviction from a cache by accumulated attention weight (no counterpart in
+ * the reference).  Of the live rows [kv_start[b], kv_len[b]) of every KV head
+ * of slot cache_slot[b] (NULL: slot b), n = min(keep, live) stay: the rows of
+ * the `recent` newest tokens (token > newest live token - recent), then those
+ * of the largest weight; equal weights: the lower row first; NaN counts as the
+ * largest.  The i-th kept row at or beyond n moves to the i-th free row below
+ * n -- K, V, weight and token -- so the rows' order is not kept (attention does
+ * not depend on it; tokens tells which is which).  Then kv_len[b] = n,
+ * kv_start[b] = 0, and weights and tokens of rows n .. old kv_len-1 become 0
+ * and -1; K and V there are left as they were.
+ *   weights (n_slots, nkv, max_seq) fp32, tokens (same) int32: a row's total
+ *   and its token's position; kv_len, kv_start (B) int32 (kv_start may be
+ *   NULL), changed in place; max_len bounds kv_len; 0 <= recent <= keep.
+ * A length or slot outside the cache, or a slot given a second time: device
+ * error 4, and that entry is left as it was.  Workspace: _workspace_size()
+ * bytes, 16-byte aligned, any contents.
+ * ---------------------------------------------------------------------- */
+QMOE_API size_t qmoe_kv_evict_workspace_size(int64_t B, int64_t nkv, int64_t max_len, int64_t keep);
+QMOE_API int qmoe_kv_evict(void* k_cache, void* v_cache, float* weights, int32_t* tokens, int32_t* kv_len,
+                           const int32_t* cache_slot, int32_t* kv_start, int64_t B, int64_t nkv, int64_t head_dim,
+                           int64_t n_slots, int64_t max_seq, int64_t max_len, int64_t keep, int64_t recent,
+                           void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
  * Expert parallelism (EP) around NCCL all-to-alls.  Rank r of n_ranks owns

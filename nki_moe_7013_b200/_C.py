@@ -58,6 +58,18 @@ _SIGNATURES = {
     "qmoe_attention_decode_workspace_size": (SZ, [I64, I64, I64]),
     "qmoe_attention_decode": (I32, [P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64,
                                     ctypes.c_float, P, P, SZ, P]),
+    "qmoe_qk_norm_rope_rows": (I32, [P, P, P, P, P, P, P, I64, I64, I64, I64, ctypes.c_float, P, P, P, P, P, I64,
+                                     I64, P]),
+    "qmoe_attention_prefix_decode_parts": (I64, [I64, I64, I64, I64, I64]),
+    "qmoe_attention_prefix_decode_workspace_size": (SZ, [I64, I64, I64, I64, I64, I32]),
+    "qmoe_attention_prefix_decode": (I32, [P, P, P, I64, I64, I64, I64, P, P, P, P, P, I64, I64, I64, I64, I64, I64,
+                                           I64, ctypes.c_float, P, I32, P, P, SZ, P]),
+    "qmoe_attention_prefix_prefill": (I32, [P, P, P, I64, I64, I64, I64, P, P, P, P, P, I64, I64, I64, I64, I64,
+                                            I64, I64, ctypes.c_float, P, P, P]),
+    "qmoe_attention_weights": (I32, [P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, ctypes.c_float, P,
+                                     I32, P]),
+    "qmoe_kv_evict_workspace_size": (SZ, [I64, I64, I64, I64]),
+    "qmoe_kv_evict": (I32, [P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, P, SZ, P]),
     "qmoe_routing_histogram": (I32, [P, I64, I64, I64, P, P]),
     "qmoe_ep_pack": (I32, [P, P, P, I64, I64, I64, I64, I64, P, P, P, P, P, P, P]),
     "qmoe_ep_unpack": (I32, [P, P, P, I64, I64, I64, I64, P, P]),

@@ -1,0 +1,462 @@
+// Decode attention over a prefix that the whole batch shares, and decode
+// attention that keeps every cache row's accumulated attention weight.
+// head_dim 128, bf16 in, fp32 scores, softmax and sums; 1 to 16 query heads
+// per KV head.
+//
+//   out_bh = softmax(c q_bh [Kp; K_b]^T) [Vp; V_b]
+//   weights[slot, g, j] (+)= sum over the heads h of group g of p_bh[j]
+//
+// over the prefix rows 0 .. P-1 (one slot of a prefix cache, the same for all
+// sequences) and the sequence's own rows kv_start[b] .. kv_len[b]-1.  Either
+// part may be empty; a row with neither gets zeros and no weight.
+//
+// The keys are cut into parts; a part yields a row's running maximum m (in
+// log2 units), its sum l of exp2(s - m) and its unnormalised output, which
+// shared_decode_combine_kernel joins:  M = max m,  out = sum_i 2^(m_i - M) o_i
+// / sum_i 2^(m_i - M) l_i.  The joined M and l also turn the scores of the
+// own rows, kept in fp32 by the first kernel, into attention weights.
+#pragma once
+
+#include "attention.cuh"
+#include "common.cuh"
+#include "flash_prefill.cuh"
+
+namespace qmoe {
+
+constexpr int kSdKeys = 64;                           // keys per stage
+constexpr int kSdHalfBytes = kSdKeys * 128;           // 64 keys x 64 dims
+constexpr int kSdTileBytes = 2 * kSdHalfBytes;        // one K or V tile: 16 KB
+constexpr int kSdStageBytes = 2 * kSdTileBytes;       // K and V
+constexpr int kSdStages = 3;
+constexpr int kSdThreads = 160;                       // 4 MMA warps, 1 producer warp
+constexpr int kSdRedStride = kAttnD + 4;
+constexpr int kSdSmemBytes = kSdStages * kSdStageBytes + 1024 + 128;
+constexpr int kSdMaxGroup = 16;                       // rows of one MMA tile
+constexpr int kSdCombineRows = 256;                   // cache rows per weight block
+static_assert(4 * 16 * kSdRedStride * 4 <= kSdStages * kSdStageBytes, "the warps are merged in the stages' memory");
+
+struct SharedDecodeArgs {
+  const __nv_bfloat16* q;
+  const int32_t* kv_len;
+  const int32_t* cache_slot;
+  const int32_t* kv_start;
+  float* part_o;    // [B*nh][nparts][128]
+  float* part_ml;   // [B*nh][nparts][2]
+  float* scores;    // [B*nkv][score_rows][G] log2-scaled scores of the own rows, or null
+  int B, nh, nkv, G, max_seq, max_len, n_slots;
+  int P, prefix_z, psplits, pchunk, row_tiles, n_prefix_units;
+  int osplits, nparts, score_rows;
+  float scale_log2;
+};
+
+// The sequence's own visible rows [lo, hi): false (device error 4) when its
+// length or slot lies outside the cache.
+__device__ __forceinline__ bool own_range(const int32_t* kv_len, const int32_t* cache_slot, const int32_t* kv_start,
+                                          int b, int max_len, int n_slots, int& slot, int& lo, int& hi) {
+  slot = cache_slot ? cache_slot[b] : b;
+  hi = kv_len[b];
+  const bool ok = hi >= 0 && hi <= max_len && slot >= 0 && slot < n_slots;
+  if (!ok) {
+    slot = 0;
+    hi = 0;
+  }
+  lo = kv_start ? max(0, min(kv_start[b], hi)) : 0;
+  return ok;
+}
+
+// One 16-byte chunk of a 128-byte-swizzled 64-column half tile.
+__device__ __forceinline__ uint32_t sw128_addr(uint32_t tile, int row, int chunk) {
+  return tile + uint32_t(chunk >> 3) * kSdHalfBytes + uint32_t(row) * 128u + (uint32_t((chunk ^ row) & 7) << 4);
+}
+__device__ __forceinline__ void ldsm_x4_at(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_trans_at(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+
+// One CTA = one part: 16 query rows of one KV head over a range of keys, read
+// once.  Rows are the heads of one sequence (own rows) or 16 consecutive
+// (sequence, head) rows of the batch (prefix).  A producer thread streams
+// 64-key K and V tiles by TMA through three 32 KB stages; four warps take 16
+// keys each (m16n8k16), each with its own running softmax, and are merged in
+// shared memory at the end.  HBM-bound: 2 CTAs per SM hold 192 KB in flight.
+// Ranges begin at their first visible row, so only a part's last tile holds
+// foreign rows: their scores are masked and their V fragments zeroed, and a
+// non-finite value there reaches nothing.
+__global__ void __launch_bounds__(kSdThreads)
+    shared_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                         const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ CUtensorMap tm_vp,
+                         const SharedDecodeArgs a) {
+  extern __shared__ uint8_t sd_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sd_smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kSdStages * kSdStageBytes);
+  uint64_t* empty = full + kSdStages;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + kSdStages);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSdStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 4);
+    }
+    *abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  const int u = blockIdx.x;
+  const bool prefix = u < a.n_prefix_units;
+  griddep_wait();
+  griddep_launch_dependents();
+  // the unit: rows row0 .. row0+n_rows-1 of (sequence, head in group) order, keys [k0, k1)
+  int kvh, part, row0, n_rows, k0, k1, z;
+  int own_b = 0;
+  if (prefix) {
+    const int rt = u % a.row_tiles, rest = u / a.row_tiles;
+    kvh = rest % a.nkv;
+    part = rest / a.nkv;
+    row0 = rt * 16;
+    n_rows = min(16, a.B * a.G - row0);
+    k0 = part * a.pchunk;
+    k1 = min(a.P, k0 + a.pchunk);
+    z = a.prefix_z + kvh;
+  } else {
+    const int v = u - a.n_prefix_units;
+    const int split = v % a.osplits, rest = v / a.osplits;
+    kvh = rest % a.nkv;
+    own_b = rest / a.nkv;
+    part = a.psplits + split;
+    row0 = own_b * a.G;
+    n_rows = a.G;
+    int slot, lo, hi;
+    if (!own_range(a.kv_len, a.cache_slot, a.kv_start, own_b, a.max_len, a.n_slots, slot, lo, hi) && threadIdx.x == 0)
+      record_device_error(kDevErrBadIndex);
+    // each sequence splits its own length, so a ragged batch leaves no split idle
+    const int chunk = ((hi - lo + a.osplits - 1) / a.osplits + kSdKeys - 1) / kSdKeys * kSdKeys;
+    k0 = min(hi, lo + split * chunk);
+    k1 = min(hi, k0 + chunk);
+    z = slot * a.nkv + kvh;
+  }
+  const int n_tiles = k1 > k0 ? (k1 - k0 + kSdKeys - 1) / kSdKeys : 0;
+  __syncthreads();
+
+  if (warp == 4) {
+    if (lane == 0 && n_tiles > 0) {
+      const CUtensorMap* mk = prefix ? &tm_kp : &tm_k;
+      const CUtensorMap* mv = prefix ? &tm_vp : &tm_v;
+      int issued = 0;
+      for (int j = 0; j < n_tiles; ++j, ++issued) {
+        const int st = j % kSdStages;
+        if (j >= kSdStages &&
+            !mbar_wait_bounded(&empty[st], (j / kSdStages - 1) & 1, abort_flag, kDevErrWaitTimeoutProducer))
+          break;
+        uint8_t* kt = smem + st * kSdStageBytes;
+        const int y = k0 + j * kSdKeys;
+        mbar_arrive_expect_tx(&full[st], kSdStageBytes);
+        tma_load_3d(kt, mk, 0, y, z, &full[st]);
+        tma_load_3d(kt + kSdHalfBytes, mk, 64, y, z, &full[st]);
+        tma_load_3d(kt + kSdTileBytes, mv, 0, y, z, &full[st]);
+        tma_load_3d(kt + kSdTileBytes + kSdHalfBytes, mv, 64, y, z, &full[st]);
+      }
+      // copies in flight land before the CTA can exit
+      for (int j = max(0, issued - kSdStages); j < issued; ++j)
+        fa_wait_landed(&full[j % kSdStages], (j / kSdStages) & 1);
+    }
+  }
+  const int g = lane >> 2, tq = lane & 3;
+  float o[16][4];
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  bool ok = true;
+  if (warp < 4) {
+    // query fragments straight from global memory; rows past n_rows are zero
+    uint32_t qa[8][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = g + 8 * h;
+      const int r = row0 + i;
+      const __nv_bfloat16* qrow = a.q + (size_t(r / a.G) * a.nh + kvh * a.G + r % a.G) * kAttnD;
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        qa[kk][h] = i < n_rows ? *reinterpret_cast<const uint32_t*>(qrow + kk * 16 + 2 * tq) : 0u;
+        qa[kk][2 + h] = i < n_rows ? *reinterpret_cast<const uint32_t*>(qrow + kk * 16 + 8 + 2 * tq) : 0u;
+      }
+    }
+#pragma unroll
+    for (int dn = 0; dn < 16; ++dn)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[dn][i] = 0.f;
+    float* sc_out = (!prefix && a.scores) ? a.scores + size_t(own_b * a.nkv + kvh) * a.score_rows * a.G : nullptr;
+    const int mi = lane >> 3, r8 = lane & 7;
+    for (int j = 0; j < n_tiles; ++j) {
+      const int st = j % kSdStages;
+      if (!fa_wait_warp(&full[st], (j / kSdStages) & 1, abort_flag, kDevErrWaitTimeoutEpilogue)) {
+        ok = false;
+        break;
+      }
+      const int key0 = k0 + j * kSdKeys + warp * 16;
+      if (key0 < k1) {
+        const uint32_t kt = smem_u32(smem + st * kSdStageBytes), vt = kt + kSdTileBytes;
+        float s[2][4];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
+#pragma unroll
+          for (int kk = 0; kk < 8; kk += 2) {
+            uint32_t b[4];
+            ldsm_x4_at(b, sw128_addr(kt, warp * 16 + nt * 8 + r8, kk * 2 + mi));
+            mma_bf16_16816(s[nt], qa[kk], b[0], b[1]);
+            mma_bf16_16816(s[nt], qa[kk + 1], b[2], b[3]);
+          }
+        }
+        const bool tail = key0 + 16 > k1;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[nt][i] *= a.scale_log2;
+            if (tail && key0 + nt * 8 + 2 * tq + (i & 1) >= k1) s[nt][i] = -INFINITY;
+          }
+        if (sc_out) {
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int key = key0 + nt * 8 + 2 * tq + (i & 1), row = g + 8 * (i >> 1);
+              if (key < k1 && row < n_rows) sc_out[size_t(key) * a.G + row] = s[nt][i];
+            }
+        }
+        float alpha[2];
+        bool grew = false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float mx = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
+          const float m_new = fmaxf(m[h], mx);
+          const float base = m_new == -INFINITY ? 0.f : m_new;
+          alpha[h] = exp2f(m[h] - base);  // m[h] == -inf -> 0
+          grew |= m_new != m[h];
+          m[h] = m_new;
+          float sum = 0.f;
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              s[nt][2 * h + e] = exp2f(s[nt][2 * h + e] - base);
+              sum += s[nt][2 * h + e];
+            }
+          l[h] = l[h] * alpha[h] + sum;
+        }
+        if (__any_sync(0xFFFFFFFFu, grew)) {
+#pragma unroll
+          for (int dn = 0; dn < 16; ++dn)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[dn][i] *= alpha[i >> 1];
+        }
+        // P in bf16 (in [0, 1], relative rounding 2^-9): the tensor core's operand type
+        uint32_t pa[4];
+        pa[0] = pack_bf16x2(s[0][0], s[0][1]);
+        pa[1] = pack_bf16x2(s[0][2], s[0][3]);
+        pa[2] = pack_bf16x2(s[1][0], s[1][1]);
+        pa[3] = pack_bf16x2(s[1][2], s[1][3]);
+        uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;  // V rows of this lane's keys
+        if (tail) {
+          const int ka = key0 + 2 * tq;
+          keep0 = (ka < k1 ? 0xFFFFu : 0u) | (ka + 1 < k1 ? 0xFFFF0000u : 0u);
+          keep1 = (ka + 8 < k1 ? 0xFFFFu : 0u) | (ka + 9 < k1 ? 0xFFFF0000u : 0u);
+        }
+#pragma unroll
+        for (int dn = 0; dn < 16; dn += 2) {
+          uint32_t bb[4];
+          ldsm_x4_trans_at(bb, sw128_addr(vt, warp * 16 + (mi & 1) * 8 + r8, dn + (mi >> 1)));
+          mma_bf16_16816(o[dn], pa, bb[0] & keep0, bb[1] & keep1);
+          mma_bf16_16816(o[dn + 1], pa, bb[2] & keep0, bb[3] & keep1);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 2);
+    }
+  }
+  // every load has landed and been read: the stages hold the warps' results now
+  const bool all_ok = __syncthreads_and(ok) != 0;
+  if (!all_ok) return;
+  float* red = reinterpret_cast<float*>(smem);
+  if (warp < 4 && n_tiles > 0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float* wr = red + (warp * 16 + g + 8 * h) * kSdRedStride;
+#pragma unroll
+      for (int dn = 0; dn < 16; ++dn)
+        *reinterpret_cast<float2*>(wr + dn * 8 + 2 * tq) = make_float2(o[dn][2 * h], o[dn][2 * h + 1]);
+      if (tq == 0) *reinterpret_cast<float2*>(wr + kAttnD) = make_float2(m[h], l[h]);
+    }
+  }
+  __syncthreads();
+  if (warp >= 4) return;
+  // eight threads per row, 16 dims each
+  const int i = threadIdx.x >> 3, d0 = (threadIdx.x & 7) * 16;
+  if (i >= n_rows) return;
+  const int r = row0 + i;
+  const size_t pidx = (size_t(r / a.G) * a.nh + kvh * a.G + r % a.G) * a.nparts + part;
+  float M = -INFINITY, L = 0.f;
+  if (n_tiles > 0) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, red[(w * 16 + i) * kSdRedStride + kAttnD]);
+    const float base = M == -INFINITY ? 0.f : M;
+    float acc[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float* rw = red + (w * 16 + i) * kSdRedStride;
+      const float sc = exp2f(rw[kAttnD] - base);
+      L += rw[kAttnD + 1] * sc;
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(rw + d0 + e);
+        acc[e] += v.x * sc;
+        acc[e + 1] += v.y * sc;
+        acc[e + 2] += v.z * sc;
+        acc[e + 3] += v.w * sc;
+      }
+    }
+    float4* po = reinterpret_cast<float4*>(a.part_o + pidx * kAttnD + d0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) po[e] = make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
+  }
+  // an empty part has l = 0; its output is not written and never read
+  if (d0 == 0) *reinterpret_cast<float2*>(a.part_ml + pidx * 2) = make_float2(M, L);
+}
+
+struct SharedCombineArgs {
+  const float* part_o;
+  const float* part_ml;
+  const float* scores;
+  const int32_t* kv_len;
+  const int32_t* cache_slot;
+  const int32_t* kv_start;
+  float* weights;   // (n_slots, nkv, max_seq) or null
+  __nv_bfloat16* out;
+  int B, nh, nkv, G, nparts, n_out_blocks, row_blocks, score_rows, max_len, max_seq, n_slots, accumulate;
+};
+
+// M and 1/l of one row from its parts, in every lane of the warp.
+__device__ __forceinline__ void join_ml(const float* part_ml, size_t base, int nparts, int lane, float& M,
+                                        float& inv_l) {
+  float mm = -INFINITY;
+  for (int s = lane; s < nparts; s += 32) mm = fmaxf(mm, part_ml[(base + s) * 2]);
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, off));
+  M = mm == -INFINITY ? 0.f : mm;
+  float L = 0.f;
+  for (int s = lane; s < nparts; s += 32) {
+    const float2 ml = *reinterpret_cast<const float2*>(part_ml + (base + s) * 2);
+    if (ml.y != 0.f) L += ml.y * exp2f(ml.x - M);
+  }
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) L += __shfl_xor_sync(0xFFFFFFFFu, L, off);
+  inv_l = L == 0.f ? 0.f : 1.f / L;
+}
+
+// Is slot of entry b also the slot of an earlier entry?  (One warp.)
+__device__ __forceinline__ bool slot_seen_before(const int32_t* cache_slot, int b, int lane) {
+  if (!cache_slot) return false;
+  const int mine = cache_slot[b];
+  bool hit = false;
+  for (int i = lane; i < b; i += 32) hit |= cache_slot[i] == mine;
+  return __any_sync(0xFFFFFFFFu, hit);
+}
+
+// Blocks [0, n_out_blocks): one warp per (sequence, head) joins the parts of
+// its output row in part order (run-to-run identical).  The blocks after
+// them: 256 own rows of one (sequence, KV head) each, one thread per row,
+// weights (+)= sum over the group's heads of exp2(s - M) / l.
+__global__ void __launch_bounds__(256) shared_decode_combine_kernel(const SharedCombineArgs a) {
+  __shared__ float sM[kSdMaxGroup], sInv[kSdMaxGroup];
+  __shared__ int s_dup;
+  griddep_wait();
+  griddep_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (int(blockIdx.x) < a.n_out_blocks) {
+    const int gw = blockIdx.x * 8 + warp;
+    if (gw >= a.B * a.nh) return;
+    const size_t base = size_t(gw) * a.nparts;
+    float M, inv;
+    join_ml(a.part_ml, base, a.nparts, lane, M, inv);
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < a.nparts; s0 += 8) {
+      float4 v[8];
+      float sc[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sc[j] = 0.f;
+        if (s0 + j < a.nparts) {
+          const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (base + s0 + j) * 2);
+          if (ml.y != 0.f) {
+            sc[j] = exp2f(ml.x - M);
+            v[j] = *reinterpret_cast<const float4*>(a.part_o + (base + s0 + j) * kAttnD + lane * 4);
+          } else {
+            v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+        } else {
+          v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        acc[0] += v[j].x * sc[j];
+        acc[1] += v[j].y * sc[j];
+        acc[2] += v[j].z * sc[j];
+        acc[3] += v[j].w * sc[j];
+      }
+    }
+    uint2 w;
+    w.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+    w.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+    *reinterpret_cast<uint2*>(a.out + size_t(gw) * kAttnD + lane * 4) = w;
+    return;
+  }
+  const int v = blockIdx.x - a.n_out_blocks;
+  const int rb = v % a.row_blocks, rest = v / a.row_blocks;
+  const int kvh = rest % a.nkv, b = rest / a.nkv;
+  int slot, lo, hi;
+  if (!own_range(a.kv_len, a.cache_slot, a.kv_start, b, a.max_len, a.n_slots, slot, lo, hi)) return;  // recorded before
+  const int first = rb * kSdCombineRows;
+  if (first >= hi) return;
+  for (int h = warp; h < a.G; h += 8) {
+    float M, inv;
+    join_ml(a.part_ml, (size_t(b) * a.nh + kvh * a.G + h) * a.nparts, a.nparts, lane, M, inv);
+    if (lane == 0) {
+      sM[h] = M;
+      sInv[h] = inv;
+    }
+  }
+  if (warp == 0) {
+    // two entries of one slot would race: the first one's weights are added
+    const bool dup = slot_seen_before(a.cache_slot, b, lane);
+    if (lane == 0) {
+      s_dup = dup;
+      if (dup) record_device_error(kDevErrBadIndex);
+    }
+  }
+  __syncthreads();
+  const int row = first + threadIdx.x;
+  if (s_dup || row >= hi) return;
+  float w = 0.f;
+  if (row >= lo) {
+    const float* sc = a.scores + (size_t(b * a.nkv + kvh) * a.score_rows + row) * a.G;
+    for (int h = 0; h < a.G; ++h) w += exp2f(sc[h] - sM[h]) * sInv[h];
+  }
+  float* dst = a.weights + (size_t(slot) * a.nkv + kvh) * a.max_seq + row;
+  *dst = a.accumulate ? *dst + w : w;
+}
+
+}  // namespace qmoe

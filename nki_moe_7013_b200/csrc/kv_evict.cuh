@@ -1,0 +1,258 @@
+// Eviction from a KV cache by accumulated attention weight.
+//
+// Of the live rows [kv_start, kv_len) of each (sequence, KV head),
+// n = min(keep, live) stay: first the rows of the `recent` newest tokens, then
+// those of the largest weight (equal weights: the lower row first; NaN counts
+// as the largest).  Attention does not depend on the order of a cache's rows
+// (a key carries its position's rotation), so nothing is shifted: the i-th
+// kept row beyond n moves into the i-th free row below n.  Sources lie at or
+// beyond n and destinations below it, so the moves need no order among
+// themselves, and an eviction of a few rows from a long cache moves only
+// these few.
+//
+// kv_evict_select_kernel (one CTA per (sequence, KV head)) finds the n-th
+// largest of the 32-bit order keys digit by digit, lists the moves, and moves
+// the rows' weights and tokens; kv_evict_move_kernel copies the K and V rows
+// over all SMs and sets the new lengths.
+#pragma once
+
+#include "attn_shared.cuh"
+#include "common.cuh"
+
+namespace qmoe {
+
+constexpr int kEvThreads = 1024;
+constexpr int kEvWarps = kEvThreads / 32;
+constexpr int kEvMaxCached = 49152;  // order keys held in shared memory (192 KB); rows past it are re-read from L2
+constexpr int kEvMoveRows = 32;      // rows per CTA of the move kernel
+
+struct EvictArgs {
+  float* weights;    // (n_slots, nkv, max_seq)
+  int32_t* tokens;   // (n_slots, nkv, max_seq)
+  int32_t* kv_len;
+  int32_t* kv_start;
+  const int32_t* cache_slot;
+  int32_t* plan;     // [B*nkv][2 + 2 * cap]: moves (-1: refused), n, source rows, destination rows
+  int B, nkv, n_slots, max_seq, max_len, keep, recent, cap, cached;
+};
+
+// Larger key = kept earlier.
+__device__ __forceinline__ uint32_t evict_key(float w, bool is_recent) {
+  if (is_recent) return 0xFFFFFFFFu;
+  if (isnan(w)) return 0xFFFFFFFEu;
+  const uint32_t u = __float_as_uint(w + 0.f);  // -0 and +0 tie
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+__global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const EvictArgs a) {
+  extern __shared__ uint32_t ev_keys[];
+  __shared__ int hist[256];
+  __shared__ int wsum[kEvWarps], wsum2[kEvWarps];
+  __shared__ int s_pick, s_rest, s_bad;
+  griddep_wait();
+  griddep_launch_dependents();
+  const int b = blockIdx.x / a.nkv, kvh = blockIdx.x % a.nkv;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int32_t* plan = a.plan + size_t(blockIdx.x) * (2 + 2 * size_t(a.cap));
+  int32_t* src = plan + 2;
+  int32_t* dst = src + a.cap;
+  int slot, lo, len;
+  const bool ok = own_range(a.kv_len, a.cache_slot, a.kv_start, b, a.max_len, a.n_slots, slot, lo, len);
+  if (warp == 0) {
+    const bool dup = ok && slot_seen_before(a.cache_slot, b, lane);
+    if (lane == 0) s_bad = !ok || dup;
+  }
+  __syncthreads();
+  if (s_bad) {  // a bad length or slot, or a slot given twice: nothing of this entry changes
+    if (tid == 0) {
+      record_device_error(kDevErrBadIndex);
+      plan[0] = -1;
+    }
+    return;
+  }
+  const int n = min(a.keep, len - lo);
+  float* w = a.weights + (size_t(slot) * a.nkv + kvh) * a.max_seq;
+  int32_t* tok = a.tokens + (size_t(slot) * a.nkv + kvh) * a.max_seq;
+
+  // the newest token
+  int newest = INT32_MIN;
+  if (a.recent > 0) {
+    for (int r = lo + tid; r < len; r += kEvThreads) newest = max(newest, tok[r]);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) newest = max(newest, __shfl_xor_sync(0xFFFFFFFFu, newest, off));
+    if (lane == 0) wsum[warp] = newest;
+    __syncthreads();
+    newest = wsum[lane];
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) newest = max(newest, __shfl_xor_sync(0xFFFFFFFFu, newest, off));
+  }
+  const long long old_most = (long long)newest - a.recent;  // tokens above it are recent
+  auto fresh_key = [&](int r) { return evict_key(w[r], a.recent > 0 && (long long)tok[r] > old_most); };
+  for (int r = lo + tid; r < min(len, a.cached); r += kEvThreads) ev_keys[r] = fresh_key(r);
+  auto key_at = [&](int r) { return r < a.cached ? ev_keys[r] : fresh_key(r); };
+  __syncthreads();
+
+  // the n-th largest key T: rows above T stay, and `take_eq` of those equal to it
+  uint32_t T = 0;
+  int take_eq = 0;
+  if (n == len - lo) {
+    take_eq = n;  // all stay (T = 0 lies below or at every key)
+  } else if (n > 0) {
+    uint32_t mask = 0;
+    int want = n;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      if (tid < 256) hist[tid] = 0;
+      __syncthreads();
+      for (int r = lo + tid; r < len; r += kEvThreads) {
+        const uint32_t k = key_at(r);
+        if ((k & mask) == T) atomicAdd(&hist[(k >> shift) & 255], 1);
+      }
+      __syncthreads();
+      if (warp == 0) {
+        // lane i holds digits 255-8i .. 248-8i, largest first
+        int c[8], sum = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          c[e] = hist[255 - lane * 8 - e];
+          sum += c[e];
+        }
+        int incl = sum;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const int t = __shfl_up_sync(0xFFFFFFFFu, incl, off);
+          if (lane >= off) incl += t;
+        }
+        int above = incl - sum;
+        if (above < want && want <= incl) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (above < want && want <= above + c[e]) {
+              s_pick = 255 - lane * 8 - e;
+              s_rest = want - above;
+            }
+            above += c[e];
+          }
+        }
+      }
+      __syncthreads();
+      T |= uint32_t(s_pick) << shift;
+      want = s_rest;
+      mask |= 0xFFu << shift;
+    }
+    take_eq = want;
+  } else {
+    T = 0xFFFFFFFFu;  // nothing stays
+  }
+  const bool all = n == len - lo;
+
+  // Each warp owns a contiguous run of rows, so ranks in row order are a scan
+  // over the warps' totals plus ballots inside the run.
+  const int run = ((len + kEvWarps - 1) / kEvWarps + 31) / 32 * 32;
+  const int r_begin = min(len, warp * run), r_end = min(len, r_begin + run);
+  int eq = 0;
+  for (int r0 = r_begin; r0 < r_end; r0 += 32) {
+    const int r = r0 + lane;
+    eq += __popc(__ballot_sync(0xFFFFFFFFu, r < r_end && r >= lo && key_at(r) == T));
+  }
+  if (lane == 0) wsum[warp] = eq;
+  __syncthreads();
+  int eq_before = 0;
+  for (int i = 0; i < warp; ++i) eq_before += wsum[i];
+  __syncthreads();
+  // two passes: count the free rows below n and the kept rows beyond it, then list them
+  int holes_before = 0, moves_before = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    int e = eq_before, holes = holes_before, moves = moves_before;
+    for (int r0 = r_begin; r0 < r_end; r0 += 32) {
+      const int r = r0 + lane;
+      const bool live = r < r_end && r >= lo;
+      const uint32_t k = live ? key_at(r) : 0u;
+      const bool is_eq = live && k == T;
+      const uint32_t eqs = __ballot_sync(0xFFFFFFFFu, is_eq);
+      const uint32_t before = (1u << lane) - 1u;
+      const bool kept = live && (all || k > T || (is_eq && e + __popc(eqs & before) < take_eq));
+      const uint32_t hs = __ballot_sync(0xFFFFFFFFu, r < r_end && r < n && !kept);
+      const uint32_t ms = __ballot_sync(0xFFFFFFFFu, kept && r >= n);
+      if (pass == 1) {
+        if (r < r_end && r < n && !kept) dst[holes + __popc(hs & before)] = r;
+        if (kept && r >= n) src[moves + __popc(ms & before)] = r;
+      }
+      e += __popc(eqs);
+      holes += __popc(hs);
+      moves += __popc(ms);
+    }
+    if (pass == 0) {
+      if (lane == 0) {
+        wsum[warp] = holes;
+        wsum2[warp] = moves;
+      }
+      __syncthreads();
+      int total = 0;
+      for (int i = 0; i < kEvWarps; ++i) {
+        if (i < warp) {
+          holes_before += wsum[i];
+          moves_before += wsum2[i];
+        }
+        total += wsum2[i];
+      }
+      if (tid == 0) {
+        plan[0] = total;
+        plan[1] = n;
+      }
+    }
+  }
+  int n_moves = 0;
+  for (int i = 0; i < kEvWarps; ++i) n_moves += wsum2[i];
+  __syncthreads();
+  for (int i = tid; i < n_moves; i += kEvThreads) {
+    const int s = src[i], d = dst[i];
+    w[d] = w[s];
+    tok[d] = tok[s];
+  }
+  __syncthreads();
+  for (int r = n + tid; r < len; r += kEvThreads) {
+    w[r] = 0.f;
+    tok[r] = -1;
+  }
+}
+
+// grid (ceil(cap / 32), B * nkv): half a warp copies one 256-byte K row and
+// one V row; the CTA's 32 rows are all loaded before the first store.
+__global__ void __launch_bounds__(256) kv_evict_move_kernel(const EvictArgs a, __nv_bfloat16* k_cache,
+                                                            __nv_bfloat16* v_cache) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int b = blockIdx.y / a.nkv, kvh = blockIdx.y % a.nkv;
+  const int32_t* plan = a.plan + size_t(blockIdx.y) * (2 + 2 * size_t(a.cap));
+  const int moves = plan[0];
+  if (moves < 0) return;
+  if (blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0) {
+    a.kv_len[b] = plan[1];
+    if (a.kv_start) a.kv_start[b] = 0;
+  }
+  const int slot = a.cache_slot ? a.cache_slot[b] : b;
+  const size_t head = (size_t(slot) * a.nkv + kvh) * a.max_seq;
+  const int sub = threadIdx.x >> 4, c = threadIdx.x & 15;
+  uint4 kr[2], vr[2];
+  int d[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int idx = blockIdx.x * kEvMoveRows + i * 16 + sub;
+    d[i] = -1;
+    if (idx < moves) {
+      const size_t s = head + plan[2 + idx];
+      d[i] = plan[2 + a.cap + idx];
+      kr[i] = reinterpret_cast<const uint4*>(k_cache + s * kAttnD)[c];
+      vr[i] = reinterpret_cast<const uint4*>(v_cache + s * kAttnD)[c];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (d[i] >= 0) {
+      reinterpret_cast<uint4*>(k_cache + (head + d[i]) * kAttnD)[c] = kr[i];
+      reinterpret_cast<uint4*>(v_cache + (head + d[i]) * kAttnD)[c] = vr[i];
+    }
+}
+
+}  // namespace qmoe

@@ -206,7 +206,8 @@ __global__ void __launch_bounds__(256)
                         const float* __restrict__ k_w, const float* __restrict__ inv_freq, int T, int nh,
                         int nkv, float eps, __nv_bfloat16* __restrict__ q_out,
                         __nv_bfloat16* __restrict__ k_cache, __nv_bfloat16* __restrict__ v_cache,
-                        int max_seq, int n_slots) {
+                        int max_seq, int n_slots, const int32_t* __restrict__ cache_rows,
+                        int32_t* __restrict__ row_tokens, float* __restrict__ row_weights) {
   __shared__ float rope_cos[kQkHeadDim / 2], rope_sin[kQkHeadDim / 2];
   griddep_wait();
   griddep_launch_dependents();
@@ -228,8 +229,17 @@ __global__ void __launch_bounds__(256)
   if (threadIdx.x < kQkHeadDim / 2)
     sincosf(float(pos) * inv_freq[threadIdx.x], &rope_sin[threadIdx.x], &rope_cos[threadIdx.x]);
   __syncthreads();
-  const bool cache_ok = slot >= 0 && slot < n_slots && pos >= 0 && pos < max_seq;
+  // the cache row: the position, or (a cache behind a prefix, or one that
+  // evicts) a row of its own
+  const int row = cache_rows ? cache_rows[t] : pos;
+  const bool cache_ok = slot >= 0 && slot < n_slots && row >= 0 && row < max_seq;
   if (!cache_ok && threadIdx.x == 0) record_device_error(kDevErrBadIndex);
+  // the row's token, and its total of attention weight so far
+  if (row_tokens && cache_ok && threadIdx.x < nkv) {
+    const size_t at = (size_t(slot) * nkv + threadIdx.x) * max_seq + row;
+    row_tokens[at] = pos;
+    row_weights[at] = 0.f;
+  }
 #pragma unroll
   for (int j = 0; j < kQkMaxHeadsPerWarp; ++j) {
     const int head = warp + j * kQkWarps;
@@ -269,7 +279,7 @@ __global__ void __launch_bounds__(256)
     } else if (cache_ok) {
       const int kvh = is_v ? head - nh - nkv : head - nh;
       __nv_bfloat16* cache = is_v ? v_cache : k_cache;
-      *reinterpret_cast<uint2*>(cache + ((size_t(slot) * nkv + kvh) * max_seq + pos) * kQkHeadDim + lane * 4) =
+      *reinterpret_cast<uint2*>(cache + ((size_t(slot) * nkv + kvh) * max_seq + row) * kQkHeadDim + lane * 4) =
           out;
     }
   }

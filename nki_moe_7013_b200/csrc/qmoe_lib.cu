@@ -6,6 +6,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -14,7 +16,11 @@
 #include <utility>
 
 #include "attention.cuh"
+#include "attn_shared.cuh"
+#include "attn_weights.cuh"
 #include "flash_prefill.cuh"
+#include "flash_prefix.cuh"
+#include "kv_evict.cuh"
 #include "blockwise.cuh"
 #include "common.cuh"
 #include "ep.cuh"
@@ -910,6 +916,79 @@ int moe_forward_on(const void* x, const void* w_router, const float* router_bias
   return launch_finalize(acc, residual, T, H, out, s);
 }
 
+// (slots * nkv, stride_rows, 128) bf16 rows as a 3D map of which the first
+// `rows` of each head are visible (rows past them read as zero); boxes of 64
+// columns x box_rows rows.
+int make_tmap_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t stride_rows, int64_t heads,
+                   int box_rows) {
+  return make_tmap_bf16_3d(map, base, 128, uint64_t(rows), uint64_t(heads), 256, uint64_t(stride_rows) * 256, 64,
+                           uint32_t(box_rows), 1);
+}
+
+// How a decode step over a shared prefix is cut into parts.
+struct SharedDecodePlan {
+  bool tc;             // the prefix part runs on the tcgen05 kernel
+  int64_t row_tiles;   // 16-row tiles, or 256-row pairs of tiles, of one KV head's rows
+  int64_t psplits, pchunk, osplits;
+};
+
+// Rows (sequences x heads of a group) above which the prefix part runs on the
+// tcgen05 kernel.
+constexpr int64_t kPrefixMmaRows = 64;
+
+SharedDecodePlan shared_decode_plan(int64_t B, int64_t G, int64_t nkv, int64_t P, int64_t max_len) {
+  SharedDecodePlan p{};
+  const int64_t sms = std::max(1, num_sms(0));
+  const int64_t rows = B * G;
+  p.tc = P > 0 && rows > kPrefixMmaRows;
+  if (p.tc) {
+    // one CTA per SM
+    const int64_t pair_rows = 2 * (qmoe::kFaRows / G * G);
+    p.row_tiles = (rows + pair_rows - 1) / pair_rows;
+    const int64_t tiles = (P + qmoe::kFaRows - 1) / qmoe::kFaRows;
+    const int64_t want = std::max<int64_t>(1, std::min(tiles, sms / (p.row_tiles * nkv)));
+    const int64_t per_part = (tiles + want - 1) / want;
+    p.pchunk = per_part * qmoe::kFaRows;
+    p.psplits = (tiles + per_part - 1) / per_part;
+  } else if (P > 0) {
+    // two CTAs per SM, parts of at least 128 keys
+    p.row_tiles = (rows + 15) / 16;
+    const int64_t want = std::max<int64_t>(
+        1, std::min((2 * sms + p.row_tiles * nkv - 1) / (p.row_tiles * nkv), (P + 127) / 128));
+    p.pchunk = ((P + want - 1) / want + qmoe::kSdKeys - 1) / qmoe::kSdKeys * qmoe::kSdKeys;
+    p.psplits = (P + p.pchunk - 1) / p.pchunk;
+  }
+  if (max_len > 0)
+    p.osplits = std::max<int64_t>(1, std::min((2 * sms + B * nkv - 1) / (B * nkv), (max_len + 127) / 128));
+  return p;
+}
+
+int check_shared_attention(const char* what, int64_t head_dim, int64_t nh, int64_t nkv, int64_t n_slots,
+                           int64_t max_seq, float scale) {
+  QMOE_REQUIRE(head_dim == qmoe::kAttnD, QMOE_ERR_UNSUPPORTED_SHAPE, "%s: head_dim must be 128", what);
+  QMOE_REQUIRE(nh > 0 && nkv > 0 && nh <= 65535 && nh % nkv == 0, QMOE_ERR_INVALID_ARGUMENT, "%s: bad heads", what);
+  QMOE_REQUIRE(nh / nkv <= qmoe::kSdMaxGroup, QMOE_ERR_UNSUPPORTED_SHAPE, "%s: more than %d query heads per KV head",
+               what, qmoe::kSdMaxGroup);
+  QMOE_REQUIRE(n_slots > 0 && max_seq > 0 && max_seq < (int64_t(1) << 30) && n_slots * nkv < (int64_t(1) << 31),
+               QMOE_ERR_INVALID_ARGUMENT, "%s: bad cache shape", what);
+  QMOE_REQUIRE(scale > 0.f && scale < INFINITY, QMOE_ERR_INVALID_ARGUMENT, "%s: scale must be positive and finite",
+               what);
+  return QMOE_OK;
+}
+
+int check_prefix(const char* what, const void* k_prefix, const void* v_prefix, int64_t n_prefix_slots,
+                 int64_t prefix_max, int64_t prefix_slot, int64_t prefix_len, int64_t nkv) {
+  QMOE_REQUIRE(prefix_len >= 0, QMOE_ERR_INVALID_ARGUMENT, "%s: bad prefix length", what);
+  if (prefix_len == 0) return QMOE_OK;
+  QMOE_REQUIRE(k_prefix && v_prefix, QMOE_ERR_INVALID_ARGUMENT, "%s: null prefix", what);
+  QMOE_REQUIRE(prefix_max < (int64_t(1) << 30) && prefix_len <= prefix_max && prefix_slot >= 0 &&
+                   prefix_slot < n_prefix_slots && n_prefix_slots * nkv < (int64_t(1) << 31),
+               QMOE_ERR_INVALID_ARGUMENT, "%s: the prefix lies outside its cache", what);
+  QMOE_REQUIRE(aligned16(k_prefix) && aligned16(v_prefix), QMOE_ERR_MISALIGNED,
+               "%s: prefix pointers must be 16-byte aligned", what);
+  return QMOE_OK;
+}
+
 }  // namespace
 
 // ---------------------------------------------------------------------------
@@ -1301,10 +1380,11 @@ int qmoe_rmsnorm(const void* x, int x_is_fp32, const void* residual, const float
                                                       static_cast<__nv_bfloat16*>(out), res_out);
 }
 
-int qmoe_qk_norm_rope(const void* qkv, const int32_t* positions, const int32_t* cache_slot,
-                      const float* q_norm_w, const float* k_norm_w, const float* inv_freq, int64_t T,
-                      int64_t nh, int64_t nkv, int64_t head_dim, float eps, void* q_out,
-                      void* k_cache, void* v_cache, int64_t n_slots, int64_t max_seq, void* stream) {
+int qmoe_qk_norm_rope_rows(const void* qkv, const int32_t* positions, const int32_t* cache_rows,
+                           const int32_t* cache_slot, const float* q_norm_w, const float* k_norm_w,
+                           const float* inv_freq, int64_t T, int64_t nh, int64_t nkv, int64_t head_dim, float eps,
+                           void* q_out, void* k_cache, void* v_cache, int32_t* row_tokens, float* row_weights,
+                           int64_t n_slots, int64_t max_seq, void* stream) {
   QMOE_REQUIRE(qkv && positions && q_norm_w && k_norm_w && inv_freq && q_out && k_cache && v_cache,
                QMOE_ERR_INVALID_ARGUMENT, "qk_norm_rope: null pointer");
   QMOE_REQUIRE(head_dim == qmoe::kQkHeadDim, QMOE_ERR_UNSUPPORTED_SHAPE,
@@ -1318,6 +1398,8 @@ int qmoe_qk_norm_rope(const void* qkv, const int32_t* positions, const int32_t* 
   QMOE_REQUIRE(aligned16(qkv) && aligned16(q_out) && aligned16(k_cache) && aligned16(v_cache) &&
                    aligned16(q_norm_w) && aligned16(k_norm_w),
                QMOE_ERR_MISALIGNED, "qk_norm_rope: pointers must be 16-byte aligned");
+  QMOE_REQUIRE((row_tokens == nullptr) == (row_weights == nullptr), QMOE_ERR_INVALID_ARGUMENT,
+               "qk_norm_rope: row_tokens and row_weights go together");
   DeviceInfo* d = nullptr;
   QMOE_CHECK(device_info(&d));
   if (T == 0) return QMOE_OK;
@@ -1327,7 +1409,15 @@ int qmoe_qk_norm_rope(const void* qkv, const int32_t* positions, const int32_t* 
                        static_cast<const __nv_bfloat16*>(qkv), positions, cache_slot, q_norm_w, k_norm_w, inv_freq,
                        int(T), int(nh), int(nkv), eps, static_cast<__nv_bfloat16*>(q_out),
                        static_cast<__nv_bfloat16*>(k_cache), static_cast<__nv_bfloat16*>(v_cache), int(max_seq),
-                       int(n_slots));
+                       int(n_slots), cache_rows, row_tokens, row_weights);
+}
+
+int qmoe_qk_norm_rope(const void* qkv, const int32_t* positions, const int32_t* cache_slot,
+                      const float* q_norm_w, const float* k_norm_w, const float* inv_freq, int64_t T,
+                      int64_t nh, int64_t nkv, int64_t head_dim, float eps, void* q_out,
+                      void* k_cache, void* v_cache, int64_t n_slots, int64_t max_seq, void* stream) {
+  return qmoe_qk_norm_rope_rows(qkv, positions, nullptr, cache_slot, q_norm_w, k_norm_w, inv_freq, T, nh, nkv,
+                                head_dim, eps, q_out, k_cache, v_cache, nullptr, nullptr, n_slots, max_seq, stream);
 }
 
 int qmoe_attention_prefill(const void* q, const void* k_cache, const void* v_cache,
@@ -1429,6 +1519,290 @@ int qmoe_attention_decode(const void* q, const void* k_cache, const void* v_cach
                        "attn_decode_combine_kernel", static_cast<const float*>(part_o),
                        static_cast<const float*>(part_ml), int(B), int(nh), int(nsplit),
                        static_cast<__nv_bfloat16*>(out));
+}
+
+int64_t qmoe_attention_prefix_decode_parts(int64_t B, int64_t nh, int64_t nkv, int64_t prefix_len, int64_t max_len) {
+  if (B <= 0 || nkv <= 0 || nh <= 0 || nh % nkv != 0) return 0;
+  const SharedDecodePlan p = shared_decode_plan(B, nh / nkv, nkv, std::max<int64_t>(prefix_len, 0),
+                                                std::max<int64_t>(max_len, 0));
+  return p.psplits + p.osplits;
+}
+
+size_t qmoe_attention_prefix_decode_workspace_size(int64_t B, int64_t nh, int64_t nkv, int64_t prefix_len,
+                                                   int64_t max_len, int with_weights) {
+  const size_t parts = size_t(qmoe_attention_prefix_decode_parts(B, nh, nkv, prefix_len, max_len));
+  if (B <= 0 || nh <= 0) return 0;
+  return size_t(B * nh) * (parts * (qmoe::kAttnD + 2) + (with_weights ? size_t(std::max<int64_t>(max_len, 0)) : 0)) *
+             sizeof(float) +
+         256;
+}
+
+int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void* v_prefix, int64_t n_prefix_slots,
+                                 int64_t prefix_max, int64_t prefix_slot, int64_t prefix_len, const void* k_cache,
+                                 const void* v_cache, const int32_t* kv_len, const int32_t* cache_slot,
+                                 const int32_t* kv_start, int64_t B, int64_t nh, int64_t nkv, int64_t head_dim,
+                                 int64_t n_slots, int64_t max_seq, int64_t max_len, float scale, float* weights,
+                                 int accumulate, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  QMOE_REQUIRE(q && k_cache && v_cache && kv_len && out && workspace, QMOE_ERR_INVALID_ARGUMENT,
+               "attention_prefix_decode: null pointer");
+  QMOE_CHECK(check_shared_attention("attention_prefix_decode", head_dim, nh, nkv, n_slots, max_seq, scale));
+  QMOE_CHECK(check_prefix("attention_prefix_decode", k_prefix, v_prefix, n_prefix_slots, prefix_max, prefix_slot,
+                          prefix_len, nkv));
+  QMOE_REQUIRE(B >= 0 && B <= 65535 && max_len >= 0 && max_len <= max_seq && (cache_slot || B <= n_slots),
+               QMOE_ERR_INVALID_ARGUMENT, "attention_prefix_decode: bad sizes");
+  QMOE_REQUIRE(workspace_bytes >= qmoe_attention_prefix_decode_workspace_size(B, nh, nkv, prefix_len, max_len,
+                                                                              weights != nullptr),
+               QMOE_ERR_WORKSPACE_TOO_SMALL, "attention_prefix_decode: workspace too small");
+  QMOE_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out) &&
+                   (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
+               QMOE_ERR_MISALIGNED, "attention_prefix_decode: pointers must be 16-byte aligned (workspace 256)");
+  DeviceInfo* d = nullptr;
+  QMOE_CHECK(device_info(&d));
+  if (B == 0) return QMOE_OK;
+  const int64_t G = nh / nkv;
+  const SharedDecodePlan p = shared_decode_plan(B, G, nkv, prefix_len, max_len);
+  const int64_t nparts = p.psplits + p.osplits;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  float* part_o = static_cast<float*>(workspace);
+  float* part_ml = part_o + size_t(B * nh * nparts) * qmoe::kAttnD;
+  float* scores = part_ml + size_t(B * nh * nparts) * 2;
+  CUtensorMap tk, tv, tkp, tvp;
+  QMOE_CHECK(make_tmap_rows(&tk, k_cache, max_seq, max_seq, n_slots * nkv, qmoe::kSdKeys));
+  QMOE_CHECK(make_tmap_rows(&tv, v_cache, max_seq, max_seq, n_slots * nkv, qmoe::kSdKeys));
+  tkp = tk;
+  tvp = tv;
+  if (p.tc) {
+    CUtensorMap tq, tk128, tv128;
+    QMOE_CHECK(make_tmap_bf16_3d(&tq, q, 128, uint64_t(nh), uint64_t(B), 256, uint64_t(nh) * 256, 64, uint32_t(G),
+                                 uint32_t(qmoe::kFaRows / G)));
+    QMOE_CHECK(make_tmap_rows(&tk128, k_prefix, prefix_len, prefix_max, n_prefix_slots * nkv, qmoe::kFaRows));
+    QMOE_CHECK(make_tmap_rows(&tv128, v_prefix, prefix_len, prefix_max, n_prefix_slots * nkv, qmoe::kFaRows));
+    qmoe::FlashPrefixArgs fa{};
+    fa.part_o = part_o;
+    fa.part_ml = part_ml;
+    fa.nh = int(nh);
+    fa.nkv = int(nkv);
+    fa.B = int(B);
+    fa.n_pairs = int(p.row_tiles);
+    fa.P = int(prefix_len);
+    fa.prefix_z = int(prefix_slot * nkv);
+    fa.G = int(G);
+    fa.nparts = int(nparts);
+    fa.tiles_per_part = int(p.pchunk / qmoe::kFaRows);
+    fa.scale_log2 = scale * 1.4426950408889634f;
+    QMOE_CHECK(set_smem(qmoe::flash_prefix_kernel<true>, qmoe::kFaSmemBytes));
+    QMOE_CHECK(launch_kernel(qmoe::flash_prefix_kernel<true>, dim3(unsigned(p.row_tiles * nkv * p.psplits)),
+                             dim3(qmoe::kFaThreads), size_t(qmoe::kFaSmemBytes), s, true, "flash_prefix_kernel", tq,
+                             tk128, tv128, tk128, tv128, fa));
+  } else if (prefix_len > 0) {
+    QMOE_CHECK(make_tmap_rows(&tkp, k_prefix, prefix_len, prefix_max, n_prefix_slots * nkv, qmoe::kSdKeys));
+    QMOE_CHECK(make_tmap_rows(&tvp, v_prefix, prefix_len, prefix_max, n_prefix_slots * nkv, qmoe::kSdKeys));
+  }
+  qmoe::SharedDecodeArgs a{};
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.kv_len = kv_len;
+  a.cache_slot = cache_slot;
+  a.kv_start = kv_start;
+  a.part_o = part_o;
+  a.part_ml = part_ml;
+  a.scores = weights ? scores : nullptr;
+  a.B = int(B);
+  a.nh = int(nh);
+  a.nkv = int(nkv);
+  a.G = int(G);
+  a.max_seq = int(max_seq);
+  a.max_len = int(max_len);
+  a.n_slots = int(n_slots);
+  a.P = int(prefix_len);
+  a.prefix_z = int(prefix_slot * nkv);
+  a.psplits = int(p.psplits);
+  a.pchunk = int(p.pchunk);
+  a.row_tiles = int(p.row_tiles);
+  a.n_prefix_units = p.tc ? 0 : int(p.row_tiles * nkv * p.psplits);
+  a.osplits = int(p.osplits);
+  a.nparts = int(nparts);
+  a.score_rows = int(max_len);
+  a.scale_log2 = scale * 1.4426950408889634f;
+  const int64_t units = a.n_prefix_units + B * nkv * p.osplits;
+  if (units > 0) {
+    QMOE_CHECK(set_smem(qmoe::shared_decode_kernel, qmoe::kSdSmemBytes));
+    QMOE_CHECK(launch_kernel(qmoe::shared_decode_kernel, dim3(unsigned(units)), dim3(qmoe::kSdThreads),
+                             size_t(qmoe::kSdSmemBytes), s, true, "shared_decode_kernel", tk, tv, tkp, tvp, a));
+  }
+  qmoe::SharedCombineArgs c{};
+  c.part_o = part_o;
+  c.part_ml = part_ml;
+  c.scores = scores;
+  c.kv_len = kv_len;
+  c.cache_slot = cache_slot;
+  c.kv_start = kv_start;
+  c.weights = weights;
+  c.out = static_cast<__nv_bfloat16*>(out);
+  c.B = int(B);
+  c.nh = int(nh);
+  c.nkv = int(nkv);
+  c.G = int(G);
+  c.nparts = int(nparts);
+  c.n_out_blocks = int((B * nh + 7) / 8);
+  c.row_blocks = int((max_len + qmoe::kSdCombineRows - 1) / qmoe::kSdCombineRows);
+  c.score_rows = int(max_len);
+  c.max_len = int(max_len);
+  c.max_seq = int(max_seq);
+  c.n_slots = int(n_slots);
+  c.accumulate = accumulate ? 1 : 0;
+  const int64_t blocks = c.n_out_blocks + (weights ? B * nkv * c.row_blocks : 0);
+  return launch_kernel(qmoe::shared_decode_combine_kernel, dim3(unsigned(blocks)), dim3(256), 0, s, true,
+                       "shared_decode_combine_kernel", c);
+}
+
+int qmoe_attention_prefix_prefill(const void* q, const void* k_prefix, const void* v_prefix, int64_t n_prefix_slots,
+                                  int64_t prefix_max, int64_t prefix_slot, int64_t prefix_len, const void* k_cache,
+                                  const void* v_cache, const int32_t* q_start, const int32_t* cache_slot,
+                                  const int32_t* kv_start, int64_t B, int64_t S, int64_t nh, int64_t nkv,
+                                  int64_t head_dim, int64_t n_slots, int64_t max_seq, float scale, void* out,
+                                  float* lse, void* stream) {
+  QMOE_REQUIRE(q && k_cache && v_cache && q_start && out, QMOE_ERR_INVALID_ARGUMENT,
+               "attention_prefix_prefill: null pointer");
+  QMOE_CHECK(check_shared_attention("attention_prefix_prefill", head_dim, nh, nkv, n_slots, max_seq, scale));
+  QMOE_CHECK(check_prefix("attention_prefix_prefill", k_prefix, v_prefix, n_prefix_slots, prefix_max, prefix_slot,
+                          prefix_len, nkv));
+  const int64_t n_pairs = (S + 2 * qmoe::kFaRows - 1) / (2 * qmoe::kFaRows);
+  QMOE_REQUIRE(B >= 0 && B <= 65535 && S >= 0 && S <= max_seq && (cache_slot || B <= n_slots),
+               QMOE_ERR_INVALID_ARGUMENT, "attention_prefix_prefill: bad sizes");
+  QMOE_REQUIRE(B * S < (int64_t(1) << 30) && n_pairs * nh * B < (int64_t(1) << 31), QMOE_ERR_INVALID_ARGUMENT,
+               "attention_prefix_prefill: too many queries");
+  QMOE_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out), QMOE_ERR_MISALIGNED,
+               "attention_prefix_prefill: pointers must be 16-byte aligned");
+  DeviceInfo* d = nullptr;
+  QMOE_CHECK(device_info(&d));
+  if (B == 0 || S == 0) return QMOE_OK;
+  CUtensorMap tq, tk, tv, tkp, tvp;
+  QMOE_CHECK(make_tmap_bf16_3d(&tq, q, 128, uint64_t(nh), uint64_t(B * S), 256, uint64_t(nh) * 256, 64, 1,
+                               qmoe::kFaRows));
+  QMOE_CHECK(make_tmap_rows(&tk, k_cache, max_seq, max_seq, n_slots * nkv, qmoe::kFaRows));
+  QMOE_CHECK(make_tmap_rows(&tv, v_cache, max_seq, max_seq, n_slots * nkv, qmoe::kFaRows));
+  tkp = tk;
+  tvp = tv;
+  if (prefix_len > 0) {
+    QMOE_CHECK(make_tmap_rows(&tkp, k_prefix, prefix_len, prefix_max, n_prefix_slots * nkv, qmoe::kFaRows));
+    QMOE_CHECK(make_tmap_rows(&tvp, v_prefix, prefix_len, prefix_max, n_prefix_slots * nkv, qmoe::kFaRows));
+  }
+  qmoe::FlashPrefixArgs a{};
+  a.q_start = q_start;
+  a.cache_slot = cache_slot;
+  a.kv_start = kv_start;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.lse = lse;
+  a.S = int(S);
+  a.nh = int(nh);
+  a.nkv = int(nkv);
+  a.max_seq = int(max_seq);
+  a.n_slots = int(n_slots);
+  a.B = int(B);
+  a.n_pairs = int(n_pairs);
+  a.P = int(prefix_len);
+  a.prefix_z = int(prefix_slot * nkv);
+  a.G = int(nh / nkv);
+  a.scale_log2 = scale * 1.4426950408889634f;
+  QMOE_CHECK(set_smem(qmoe::flash_prefix_kernel<false>, qmoe::kFaSmemBytes));
+  return launch_kernel(qmoe::flash_prefix_kernel<false>, dim3(unsigned(n_pairs * nh * B)), dim3(qmoe::kFaThreads),
+                       size_t(qmoe::kFaSmemBytes), static_cast<cudaStream_t>(stream), true, "flash_prefix_kernel", tq,
+                       tk, tv, tkp, tvp, a);
+}
+
+int qmoe_attention_weights(const void* q, const float* lse, const void* k_cache, const int32_t* q_start,
+                           const int32_t* cache_slot, const int32_t* kv_start, int64_t B, int64_t S, int64_t nh,
+                           int64_t nkv, int64_t head_dim, int64_t n_slots, int64_t max_seq, int64_t max_len,
+                           float scale, float* weights, int accumulate, void* stream) {
+  QMOE_REQUIRE(q && lse && k_cache && q_start && weights, QMOE_ERR_INVALID_ARGUMENT,
+               "attention_weights: null pointer");
+  QMOE_CHECK(check_shared_attention("attention_weights", head_dim, nh, nkv, n_slots, max_seq, scale));
+  QMOE_REQUIRE(B >= 0 && B <= 65535 && S >= 0 && S <= max_len && max_len <= max_seq && (cache_slot || B <= n_slots),
+               QMOE_ERR_INVALID_ARGUMENT, "attention_weights: bad sizes");
+  const int64_t blocks = (max_len + qmoe::kFaRows - 1) / qmoe::kFaRows * nkv * B;
+  QMOE_REQUIRE(B * S < (int64_t(1) << 30) && blocks < (int64_t(1) << 31), QMOE_ERR_INVALID_ARGUMENT,
+               "attention_weights: too many queries");
+  QMOE_REQUIRE(aligned16(q) && aligned16(k_cache), QMOE_ERR_MISALIGNED,
+               "attention_weights: pointers must be 16-byte aligned");
+  DeviceInfo* d = nullptr;
+  QMOE_CHECK(device_info(&d));
+  if (B == 0 || S == 0) return QMOE_OK;
+  const int64_t G = nh / nkv;
+  CUtensorMap tq, tk;
+  QMOE_CHECK(make_tmap_bf16_3d(&tq, q, 128, uint64_t(nh), uint64_t(B * S), 256, uint64_t(nh) * 256, 64, uint32_t(G),
+                               uint32_t(qmoe::kFaRows / G)));
+  QMOE_CHECK(make_tmap_rows(&tk, k_cache, max_seq, max_seq, n_slots * nkv, qmoe::kFaRows));
+  qmoe::AttnWeightsArgs a{};
+  a.lse = lse;
+  a.q_start = q_start;
+  a.cache_slot = cache_slot;
+  a.kv_start = kv_start;
+  a.weights = weights;
+  a.B = int(B);
+  a.S = int(S);
+  a.nh = int(nh);
+  a.nkv = int(nkv);
+  a.G = int(G);
+  a.n_slots = int(n_slots);
+  a.max_seq = int(max_seq);
+  a.max_len = int(max_len);
+  a.accumulate = accumulate ? 1 : 0;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  QMOE_CHECK(set_smem(qmoe::attn_weights_kernel, qmoe::kAwSmemBytes));
+  return launch_kernel(qmoe::attn_weights_kernel, dim3(unsigned(blocks)), dim3(qmoe::kAwThreads),
+                       size_t(qmoe::kAwSmemBytes), static_cast<cudaStream_t>(stream), true, "attn_weights_kernel", tq,
+                       tk, a);
+}
+
+size_t qmoe_kv_evict_workspace_size(int64_t B, int64_t nkv, int64_t max_len, int64_t keep) {
+  if (B <= 0 || nkv <= 0 || max_len < 0 || keep < 0) return 0;
+  return size_t(B * nkv) * (2 + 2 * size_t(std::min(keep, max_len))) * sizeof(int32_t);
+}
+
+int qmoe_kv_evict(void* k_cache, void* v_cache, float* weights, int32_t* tokens, int32_t* kv_len,
+                  const int32_t* cache_slot, int32_t* kv_start, int64_t B, int64_t nkv, int64_t head_dim,
+                  int64_t n_slots, int64_t max_seq, int64_t max_len, int64_t keep, int64_t recent, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+  QMOE_REQUIRE(k_cache && v_cache && weights && tokens && kv_len && workspace, QMOE_ERR_INVALID_ARGUMENT,
+               "kv_evict: null pointer");
+  QMOE_REQUIRE(head_dim == qmoe::kAttnD, QMOE_ERR_UNSUPPORTED_SHAPE, "kv_evict: head_dim must be 128");
+  QMOE_REQUIRE(nkv > 0 && n_slots > 0 && max_seq > 0 && max_seq < (int64_t(1) << 30) && max_len >= 0 &&
+                   max_len <= max_seq && B >= 0 && B * nkv <= 65535 && (cache_slot || B <= n_slots),
+               QMOE_ERR_INVALID_ARGUMENT, "kv_evict: bad sizes");
+  QMOE_REQUIRE(keep >= 0 && recent >= 0 && recent <= keep && keep < (int64_t(1) << 30), QMOE_ERR_INVALID_ARGUMENT,
+               "kv_evict: needs 0 <= recent <= keep");
+  QMOE_REQUIRE(workspace_bytes >= qmoe_kv_evict_workspace_size(B, nkv, max_len, keep), QMOE_ERR_WORKSPACE_TOO_SMALL,
+               "kv_evict: workspace too small");
+  QMOE_REQUIRE(aligned16(k_cache) && aligned16(v_cache) && aligned16(workspace), QMOE_ERR_MISALIGNED,
+               "kv_evict: pointers must be 16-byte aligned");
+  DeviceInfo* d = nullptr;
+  QMOE_CHECK(device_info(&d));
+  if (B == 0) return QMOE_OK;
+  qmoe::EvictArgs a{};
+  a.weights = weights;
+  a.tokens = tokens;
+  a.kv_len = kv_len;
+  a.kv_start = kv_start;
+  a.cache_slot = cache_slot;
+  a.plan = static_cast<int32_t*>(workspace);
+  a.B = int(B);
+  a.nkv = int(nkv);
+  a.n_slots = int(n_slots);
+  a.max_seq = int(max_seq);
+  a.max_len = int(max_len);
+  a.keep = int(keep);
+  a.recent = int(recent);
+  a.cap = int(std::min(keep, max_len));
+  a.cached = int(std::min<int64_t>(max_len, qmoe::kEvMaxCached));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int smem = a.cached * 4;
+  QMOE_CHECK(set_smem(qmoe::kv_evict_select_kernel, std::max(smem, 1024)));
+  QMOE_CHECK(launch_kernel(qmoe::kv_evict_select_kernel, dim3(unsigned(B * nkv)), dim3(qmoe::kEvThreads),
+                           size_t(smem), s, true, "kv_evict_select_kernel", a));
+  const int64_t move_blocks = std::max<int64_t>(1, (a.cap + qmoe::kEvMoveRows - 1) / qmoe::kEvMoveRows);
+  return launch_kernel(qmoe::kv_evict_move_kernel, dim3(unsigned(move_blocks), unsigned(B * nkv)), dim3(256), 0, s,
+                       true, "kv_evict_move_kernel", a, static_cast<__nv_bfloat16*>(k_cache),
+                       static_cast<__nv_bfloat16*>(v_cache));
 }
 
 int qmoe_routing_histogram(const int32_t* topk_idx, int64_t T, int64_t k, int64_t E, int32_t* chunk_hist,

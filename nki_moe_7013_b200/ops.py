@@ -541,24 +541,39 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Optiona
 def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, q_norm_w: torch.Tensor,
                  k_norm_w: torch.Tensor, inv_freq: torch.Tensor, nh: int, nkv: int, eps: float,
                  k_cache: torch.Tensor, v_cache: torch.Tensor,
-                 cache_slot: Optional[torch.Tensor] = None) -> torch.Tensor:
+                 cache_slot: Optional[torch.Tensor] = None, cache_rows: Optional[torch.Tensor] = None,
+                 row_tokens: Optional[torch.Tensor] = None,
+                 row_weights: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Fused per-head QK-RMSNorm + RoPE; appends K/V into the caches.
-    Returns q (T, nh, 128) bf16."""
+    Returns q (T, nh, 128) bf16.  ``cache_rows`` (T,) int32: the cache row of
+    each token where it is not its position (a cache behind a shared prefix,
+    a cache that evicts).  ``row_tokens`` / ``row_weights`` (n_slots, nkv,
+    max_seq) int32 / fp32, both or neither: the appended rows' entries are set
+    to the position and 0."""
     _need(qkv, "qkv", torch.bfloat16, 2)
     _need(positions, "positions", torch.int32, 1)
     _need(k_cache, "k_cache", torch.bfloat16, 4)
     _need(v_cache, "v_cache", torch.bfloat16, 4)
     if cache_slot is not None:
         _need(cache_slot, "cache_slot", torch.int32, 1)
+    if cache_rows is not None:
+        _need(cache_rows, "cache_rows", torch.int32, 1)
+        if cache_rows.shape[0] != qkv.shape[0]:
+            raise ValueError("cache_rows must hold one row per token")
+    if (row_tokens is None) != (row_weights is None):
+        raise ValueError("row_tokens and row_weights go together")
+    if row_tokens is not None:
+        _need_rows(row_tokens, "row_tokens", torch.int32, k_cache)
+        _need_rows(row_weights, "row_weights", torch.float32, k_cache)
     T = qkv.shape[0]
     hd = k_cache.shape[3]
     dev = qkv.device
     q = torch.empty((T, nh, hd), dtype=torch.bfloat16, device=dev)
     with torch.cuda.device(dev):
-        _C.check(_C.lib().qmoe_qk_norm_rope(
-            _ptr(qkv), _ptr(positions), _ptr(cache_slot), _ptr(q_norm_w), _ptr(k_norm_w), _ptr(inv_freq),
-            T, nh, nkv, hd, float(eps), _ptr(q), _ptr(k_cache), _ptr(v_cache), k_cache.shape[0],
-            k_cache.shape[2], _stream(dev)), "qmoe_qk_norm_rope")
+        _C.check(_C.lib().qmoe_qk_norm_rope_rows(
+            _ptr(qkv), _ptr(positions), _ptr(cache_rows), _ptr(cache_slot), _ptr(q_norm_w), _ptr(k_norm_w),
+            _ptr(inv_freq), T, nh, nkv, hd, float(eps), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(row_tokens),
+            _ptr(row_weights), k_cache.shape[0], k_cache.shape[2], _stream(dev)), "qmoe_qk_norm_rope")
     return q
 
 
@@ -613,6 +628,237 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
             workspace.numel(), _stream(dev)),
             "qmoe_attention_decode")
     return out
+
+
+# ----------------------------------------------------------------------------
+# shared prefixes and bounded caches
+# ----------------------------------------------------------------------------
+
+def _need_rows(t: torch.Tensor, name: str, dtype, k_cache: torch.Tensor):
+    """A per-row array (n_slots, nkv, max_seq) of a cache."""
+    _need(t, name, dtype, 3)
+    if tuple(t.shape) != tuple(k_cache.shape[:3]):
+        raise ValueError(f"{name} must be {tuple(k_cache.shape[:3])} like the cache's rows (got {tuple(t.shape)})")
+    if t.device != k_cache.device:
+        raise ValueError(f"{name} must be on the cache's device")
+
+
+def _need_cache(k: torch.Tensor, v: Optional[torch.Tensor], what: str = "cache"):
+    _need(k, f"k_{what}", torch.bfloat16, 4)
+    if v is not None:
+        _need(v, f"v_{what}", torch.bfloat16, 4)
+        if v.shape != k.shape or v.device != k.device:
+            raise ValueError(f"k_{what} and v_{what} must have one shape and device")
+
+
+def _need_i32(t: Optional[torch.Tensor], name: str, n: int, dev):
+    if t is None:
+        return
+    _need(t, name, torch.int32, 1)
+    if t.shape[0] != n or t.device != dev:
+        raise ValueError(f"{name} must hold {n} int32 on {dev}")
+
+
+def _need_prefix(k_prefix, v_prefix, prefix_len: int, prefix_slot: int, k_cache: torch.Tensor):
+    """(pointer, pointer, slots, rows per slot) of a prefix; nulls without one."""
+    if prefix_len == 0:
+        return None, None, 0, 0
+    if k_prefix is None or v_prefix is None:
+        raise ValueError("a prefix of more than 0 rows needs k_prefix and v_prefix")
+    _need_cache(k_prefix, v_prefix, "prefix")
+    if k_prefix.shape[1] != k_cache.shape[1] or k_prefix.shape[3] != k_cache.shape[3] or \
+            k_prefix.device != k_cache.device:
+        raise ValueError("the prefix must have the cache's KV heads, head dim and device")
+    return _ptr(k_prefix), _ptr(v_prefix), k_prefix.shape[0], k_prefix.shape[2]
+
+
+def _need_heads(q: torch.Tensor, rows: int, k_cache: torch.Tensor):
+    _need(q, "q", torch.bfloat16, 3)
+    if q.shape[0] != rows or q.shape[2] != k_cache.shape[3] or q.device != k_cache.device:
+        raise ValueError(f"q must be ({rows}, heads, {k_cache.shape[3]}) on the cache's device "
+                         f"(got {tuple(q.shape)} on {q.device})")
+
+
+def _need_batch(B: int, cache_slot: Optional[torch.Tensor], k_cache: torch.Tensor):
+    if cache_slot is None and B > k_cache.shape[0]:
+        raise ValueError(f"{B} sequences in a cache of {k_cache.shape[0]} slots need cache_slot")
+
+
+def attention_prefix_decode(q: torch.Tensor, k_prefix: Optional[torch.Tensor], v_prefix: Optional[torch.Tensor],
+                            prefix_len: int, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_len: torch.Tensor,
+                            max_len: int, scale: Optional[float] = None,
+                            cache_slot: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                            kv_start: Optional[torch.Tensor] = None, prefix_slot: int = 0,
+                            weights: Optional[torch.Tensor] = None, accumulate: bool = True) -> torch.Tensor:
+    """Decode attention for a batch that shares a prefix; q (B, nh, 128) ->
+    (B, nh*128) bf16.  Each sequence sees rows 0 .. prefix_len-1 of slot
+    ``prefix_slot`` of k_prefix / v_prefix (n, nkv, rows, 128), read once for
+    the batch, and its own cache rows kv_start .. kv_len-1.  ``max_len``
+    bounds kv_len.  1 to 16 query heads per KV head.
+    ``weights`` (n_slots, nkv, max_seq) fp32: every own row's attention
+    probability, summed over the query heads of its KV head, is added to it
+    (``accumulate=False``: replaces it)."""
+    _need_cache(k_cache, v_cache)
+    _need(kv_len, "kv_len", torch.int32, 1)
+    B = kv_len.shape[0]
+    _need_heads(q, B, k_cache)
+    nh, hd = q.shape[1], q.shape[2]
+    dev = k_cache.device
+    _need_i32(kv_len, "kv_len", B, dev)
+    _need_i32(cache_slot, "cache_slot", B, dev)
+    _need_i32(kv_start, "kv_start", B, dev)
+    _need_batch(B, cache_slot, k_cache)
+    kp, vp, n_prefix, prefix_max = _need_prefix(k_prefix, v_prefix, prefix_len, prefix_slot, k_cache)
+    if weights is not None:
+        _need_rows(weights, "weights", torch.float32, k_cache)
+    n_slots, nkv, max_seq = k_cache.shape[:3]
+    scale = hd ** -0.5 if scale is None else scale
+    lib = _C.lib()
+    out = torch.empty((B, nh * hd), dtype=torch.bfloat16, device=dev)
+    if B == 0:
+        return out
+    with torch.cuda.device(dev):
+        ws_bytes = int(lib.qmoe_attention_prefix_decode_workspace_size(B, nh, nkv, prefix_len, max_len,
+                                                                       0 if weights is None else 1))
+        if workspace is None or workspace.numel() < ws_bytes:
+            workspace = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
+        _C.check(lib.qmoe_attention_prefix_decode(
+            _ptr(q), kp, vp, n_prefix, prefix_max, prefix_slot, prefix_len, _ptr(k_cache), _ptr(v_cache),
+            _ptr(kv_len), _ptr(cache_slot), _ptr(kv_start), B, nh, nkv, hd, n_slots, max_seq, max_len, float(scale),
+            _ptr(weights), 1 if accumulate else 0, _ptr(out), _ptr(workspace), workspace.numel(), _stream(dev)),
+            "qmoe_attention_prefix_decode")
+    return out
+
+
+def attention_prefix_decode_workspace_size(B: int, nh: int, nkv: int, prefix_len: int, max_len: int,
+                                           with_weights: bool = False) -> int:
+    """Bytes of the ``workspace`` of attention_prefix_decode / _decode_weights
+    (prefix_len 0) on the current device."""
+    return int(_C.lib().qmoe_attention_prefix_decode_workspace_size(B, nh, nkv, prefix_len, max_len,
+                                                                    1 if with_weights else 0))
+
+
+def attention_decode_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_len: torch.Tensor,
+                             max_len: int, weights: torch.Tensor, accumulate: bool = True,
+                             scale: Optional[float] = None, cache_slot: Optional[torch.Tensor] = None,
+                             workspace: Optional[torch.Tensor] = None,
+                             kv_start: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """attention_decode that also adds every cache row's attention probability,
+    summed over the query heads of its KV head, to ``weights`` (n_slots, nkv,
+    max_seq) fp32 (``accumulate=False``: replaces it).  A cache slot may occur
+    once per call."""
+    if weights is None:
+        raise TypeError("weights must be a tensor")
+    return attention_prefix_decode(q, None, None, 0, k_cache, v_cache, kv_len, max_len, scale=scale,
+                                   cache_slot=cache_slot, workspace=workspace, kv_start=kv_start, weights=weights,
+                                   accumulate=accumulate)
+
+
+def attention_prefix_prefill(q: torch.Tensor, k_prefix: Optional[torch.Tensor], v_prefix: Optional[torch.Tensor],
+                             prefix_len: int, k_cache: torch.Tensor, v_cache: torch.Tensor, q_start: torch.Tensor,
+                             B: int, S: int, scale: Optional[float] = None,
+                             cache_slot: Optional[torch.Tensor] = None, kv_start: Optional[torch.Tensor] = None,
+                             prefix_slot: int = 0, return_lse: bool = False):
+    """attention_prefill behind a shared prefix: query i of sequence b sees the
+    prefix rows 0 .. prefix_len-1 (of slot ``prefix_slot``) and its own cache
+    rows kv_start .. q_start + i; q (B*S, nh, 128) -> (B*S, nh*128) bf16.  A
+    query before kv_start (padding) gets zeros.  With ``return_lse`` also the
+    log-sum-exp (B*S, nh) fp32 of each row's scores (-inf for padding), which
+    attention_weights takes.  prefix_len 0: no prefix."""
+    _need_cache(k_cache, v_cache)
+    _need_heads(q, B * S, k_cache)
+    nh, hd = q.shape[1], q.shape[2]
+    dev = k_cache.device
+    _need(q_start, "q_start", torch.int32, 1)
+    _need_i32(q_start, "q_start", B, dev)
+    _need_i32(cache_slot, "cache_slot", B, dev)
+    _need_i32(kv_start, "kv_start", B, dev)
+    _need_batch(B, cache_slot, k_cache)
+    kp, vp, n_prefix, prefix_max = _need_prefix(k_prefix, v_prefix, prefix_len, prefix_slot, k_cache)
+    n_slots, nkv, max_seq = k_cache.shape[:3]
+    scale = hd ** -0.5 if scale is None else scale
+    out = torch.empty((B * S, nh * hd), dtype=torch.bfloat16, device=dev)
+    lse = torch.empty((B * S, nh), dtype=torch.float32, device=dev) if return_lse else None
+    if B * S == 0:
+        return (out, lse) if return_lse else out
+    with torch.cuda.device(dev):
+        _C.check(_C.lib().qmoe_attention_prefix_prefill(
+            _ptr(q), kp, vp, n_prefix, prefix_max, prefix_slot, prefix_len, _ptr(k_cache), _ptr(v_cache),
+            _ptr(q_start), _ptr(cache_slot), _ptr(kv_start), B, S, nh, nkv, hd, n_slots, max_seq, float(scale),
+            _ptr(out), _ptr(lse), _stream(dev)), "qmoe_attention_prefix_prefill")
+    return (out, lse) if return_lse else out
+
+
+def attention_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, q_start: torch.Tensor, B: int, S: int,
+                      weights: torch.Tensor, accumulate: bool = True, scale: Optional[float] = None,
+                      cache_slot: Optional[torch.Tensor] = None, kv_start: Optional[torch.Tensor] = None,
+                      max_len: Optional[int] = None) -> torch.Tensor:
+    """Attention weights of S queries per sequence, summed per own cache row:
+    ``weights`` (n_slots, nkv, max_seq) fp32 += (``accumulate=False``: =) the
+    sum over the queries and the KV head's query heads of exp(scale q.k - lse).
+    ``q`` (B*S, nh, 128) and ``lse`` (B*S, nh) as of attention_prefix_prefill
+    (or the rows of a prompt's last S queries).  A cache slot may occur once
+    per call.  ``max_len``: a bound on q_start + S (default: the cache's rows).
+    Returns weights."""
+    _need_cache(k_cache, None)
+    _need_heads(q, B * S, k_cache)
+    nh, hd = q.shape[1], q.shape[2]
+    dev = k_cache.device
+    _need(lse, "lse", torch.float32, 2)
+    if tuple(lse.shape) != (B * S, nh) or lse.device != dev:
+        raise ValueError(f"lse must be ({B * S}, {nh}) on the cache's device")
+    _need(q_start, "q_start", torch.int32, 1)
+    _need_i32(q_start, "q_start", B, dev)
+    _need_i32(cache_slot, "cache_slot", B, dev)
+    _need_i32(kv_start, "kv_start", B, dev)
+    _need_batch(B, cache_slot, k_cache)
+    _need_rows(weights, "weights", torch.float32, k_cache)
+    n_slots, nkv, max_seq = k_cache.shape[:3]
+    scale = hd ** -0.5 if scale is None else scale
+    if B * S == 0:
+        return weights
+    with torch.cuda.device(dev):
+        _C.check(_C.lib().qmoe_attention_weights(
+            _ptr(q), _ptr(lse), _ptr(k_cache), _ptr(q_start), _ptr(cache_slot), _ptr(kv_start), B, S, nh, nkv, hd,
+            n_slots, max_seq, max_seq if max_len is None else max_len, float(scale), _ptr(weights),
+            1 if accumulate else 0, _stream(dev)), "qmoe_attention_weights")
+    return weights
+
+
+def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, tokens: torch.Tensor,
+             kv_len: torch.Tensor, max_len: int, keep: int, recent: int = 0,
+             cache_slot: Optional[torch.Tensor] = None, kv_start: Optional[torch.Tensor] = None,
+             workspace: Optional[torch.Tensor] = None) -> None:
+    """Brings each sequence's cache down to min(keep, live) rows per KV head,
+    in place: the rows of the ``recent`` newest tokens stay, then those of the
+    largest ``weights`` (n_slots, nkv, max_seq) fp32 (equal: the lower row).
+    ``tokens`` (n_slots, nkv, max_seq) int32 holds each row's position.  Kept
+    rows beyond the new length move -- with their weight and token -- into free
+    rows below it, so the rows' order changes; kv_len (B,) becomes the new
+    length and kv_start (B,) 0, both on the device.  ``max_len`` bounds
+    kv_len.  A cache slot may occur once per call."""
+    _need_cache(k_cache, v_cache)
+    dev = k_cache.device
+    _need(kv_len, "kv_len", torch.int32, 1)
+    B = kv_len.shape[0]
+    _need_i32(kv_len, "kv_len", B, dev)
+    _need_i32(cache_slot, "cache_slot", B, dev)
+    _need_i32(kv_start, "kv_start", B, dev)
+    _need_batch(B, cache_slot, k_cache)
+    _need_rows(weights, "weights", torch.float32, k_cache)
+    _need_rows(tokens, "tokens", torch.int32, k_cache)
+    n_slots, nkv, max_seq, hd = k_cache.shape
+    if B == 0:
+        return
+    lib = _C.lib()
+    ws_bytes = int(lib.qmoe_kv_evict_workspace_size(B, nkv, max_len, keep))
+    if workspace is None or workspace.numel() < ws_bytes:
+        workspace = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        _C.check(lib.qmoe_kv_evict(
+            _ptr(k_cache), _ptr(v_cache), _ptr(weights), _ptr(tokens), _ptr(kv_len), _ptr(cache_slot),
+            _ptr(kv_start), B, nkv, hd, n_slots, max_seq, max_len, keep, recent, _ptr(workspace),
+            workspace.numel(), _stream(dev)), "qmoe_kv_evict")
 
 
 # ----------------------------------------------------------------------------
