@@ -17,9 +17,21 @@ only on the difference of two positions the attention output is the same up
 to fp32 rounding.  Padding query rows get a zero attention output.  Any
 other mask (holes, right padding, 4D) is refused with a ValueError.
 
+``prefix`` (a ``SharedPrefix``): rows that every sequence of the batch sees
+before its own -- a system prompt stored once, in a cache of its own, instead
+of in every slot.  New tokens sit at positions ``prefix.length`` + their own
+(left padding not counted), and both attention forms read the prefix once for
+the batch.
+
+A cache made with ``track=True`` also holds, for every row and KV head, the
+attention weight it has received so far and its token's position; its
+``evict(keep, recent)`` brings it down to ``keep`` rows per KV head, the most
+recent ones and those of the largest weight, and later tokens are appended
+behind them at their true positions.
+
 All kernels come from the CUDA library: tcgen05 projections (``ops.linear``),
 the fused QK-norm + RoPE + cache append, flash-prefill / split-KV
-flash-decode.
+flash-decode, their forms over a shared prefix, and the eviction.
 """
 from __future__ import annotations
 
@@ -42,14 +54,38 @@ class KVCache:
     """K and V caches (slots, nkv, max_seq, head_dim) bf16 plus per-slot lengths.
 
     ``lengths`` is kept on the host (it drives shapes and launch sizes) and
-    mirrored on the device for the kernels."""
+    mirrored on the device for the kernels.
 
-    def __init__(self, n_slots: int, nkv: int, max_seq: int, head_dim: int, device="cuda"):
+    ``track``: the cache can evict.  It then holds every row's accumulated
+    attention weight (``weights``, fp32) and its token's position (``tokens``,
+    int32), both (slots, nkv, max_seq); each KV head keeps rows of its own, so
+    after an eviction the heads' rows hold different tokens.  Calls with
+    several new tokens add the weights of the last ``score_queries`` of them
+    (None: of all)."""
+
+    def __init__(self, n_slots: int, nkv: int, max_seq: int, head_dim: int, device="cuda", track: bool = False,
+                 score_queries: Optional[int] = None):
+        if score_queries is not None and score_queries < 1:
+            raise ValueError("score_queries must be at least 1")
         self.k = torch.zeros((n_slots, nkv, max_seq, head_dim), dtype=torch.bfloat16, device=device)
         self.v = torch.zeros_like(self.k)
         self.lengths: List[int] = [0] * n_slots
         self.pad: List[int] = [0] * n_slots      # leading padding rows per slot
+        self._clear_positions(n_slots)
         self.max_seq = max_seq
+        self.score_queries = score_queries
+        self.weights = torch.zeros(self.k.shape[:3], dtype=torch.float32, device=device) if track else None
+        self.tokens = (torch.full(self.k.shape[:3], -1, dtype=torch.int32, device=device) if track else None)
+
+    def _clear_positions(self, n_slots: int) -> None:
+        self.offset: List[int] = [0] * n_slots      # a new row's position less the row
+        self.prefix_len: List[int] = [0] * n_slots  # rows of the shared prefix the slot was filled behind
+        self.lead: List[int] = [0] * n_slots        # leading paddings the slot was filled with
+        self.dropped: List[int] = [0] * n_slots     # rows evicted so far
+
+    @property
+    def tracked(self) -> bool:
+        return self.weights is not None
 
     @property
     def n_slots(self) -> int:
@@ -63,13 +99,65 @@ class KVCache:
         self.v[:, :, :length].normal_(generator=g)
         self.lengths = [length] * self.n_slots
         self.pad = [0] * self.n_slots
+        self._clear_positions(self.n_slots)
+        if self.tracked:
+            self.weights.zero_()
+            self.tokens.fill_(-1)
+            self.tokens[:, :, :length] = torch.arange(length, dtype=torch.int32, device=self.k.device)
         return self
 
     def reset(self) -> "KVCache":
         """Empty every slot (the contents are overwritten by the next appends)."""
         self.lengths = [0] * self.n_slots
         self.pad = [0] * self.n_slots
+        self._clear_positions(self.n_slots)
         return self
+
+    def as_prefix(self, slot: int = 0) -> "SharedPrefix":
+        """The rows of one slot as a prefix for other sequences (no copy: the
+        slot must not change while the prefix is in use)."""
+        if not 0 <= slot < self.n_slots:
+            raise ValueError(f"slot {slot} of a cache of {self.n_slots}")
+        if self.pad[slot] or self.offset[slot] or self.dropped[slot]:
+            raise ValueError("a padded slot, one behind a prefix or one that evicted rows cannot be a prefix")
+        return SharedPrefix(self.k, self.v, self.lengths[slot], slot)
+
+    def evict(self, keep: int, recent: int = 0) -> "KVCache":
+        """Bring every slot down to min(keep, its tokens) rows per KV head: the
+        ``recent`` newest tokens and those of the largest accumulated weight
+        (``ops.kv_evict``).  Paddings leave; the rows' order changes."""
+        if not self.tracked:
+            raise ValueError("only a cache made with track=True can evict")
+        if not 0 <= recent <= keep:
+            raise ValueError("evict needs 0 <= recent <= keep")
+        dev = self.k.device
+        kv_len = torch.tensor(self.lengths, dtype=torch.int32).to(dev, non_blocking=True)
+        start = torch.tensor(self.pad, dtype=torch.int32).to(dev, non_blocking=True) if any(self.pad) else None
+        ops.kv_evict(self.k, self.v, self.weights, self.tokens, kv_len, max(self.lengths), keep, recent=recent,
+                     kv_start=start)
+        self._evicted(keep)
+        return self
+
+    def _evicted(self, keep: int) -> None:
+        """The host's side of an eviction: lengths, paddings, and the distance
+        of a new row's position from the row."""
+        for b, n in enumerate(self.lengths):
+            self.lengths[b] = min(keep, n - self.pad[b])
+            self.offset[b] += n - self.lengths[b]
+            self.dropped[b] += n - self.lengths[b]
+            self.pad[b] = 0
+
+
+@dataclass
+class SharedPrefix:
+    """Rows 0 .. length-1 of slot ``slot`` of a K / V cache (n, nkv, rows, 128)
+    bf16, rotated for positions 0 .. length-1, that every sequence of a batch
+    sees before its own rows."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    length: int
+    slot: int = 0
 
 
 def left_padding(attention_mask: Optional[torch.Tensor], B: int, S: int, L0: List[int]) -> Optional[List[int]]:
@@ -175,12 +263,14 @@ class Qwen3MoeAttention(nn.Module):
         self.inv_freq = rope_inv_freq(cfg.head_dim, cfg.rope_theta, self.w.wqkv.device)
         self._decode_ws: Optional[torch.Tensor] = None
 
-    def new_cache(self, n_slots: int, max_seq: int) -> KVCache:
-        return KVCache(n_slots, self.cfg.num_key_value_heads, max_seq, self.cfg.head_dim, self.w.wqkv.device)
+    def new_cache(self, n_slots: int, max_seq: int, track: bool = False,
+                  score_queries: Optional[int] = None) -> KVCache:
+        return KVCache(n_slots, self.cfg.num_key_value_heads, max_seq, self.cfg.head_dim, self.w.wqkv.device,
+                       track=track, score_queries=score_queries)
 
     def forward(self, hidden_states: torch.Tensor, position_ids: Optional[torch.Tensor] = None,
                 past_key_value: Optional[KVCache] = None, timer: Optional[StageTimer] = None,
-                attention_mask: Optional[torch.Tensor] = None):
+                attention_mask: Optional[torch.Tensor] = None, prefix: Optional[SharedPrefix] = None):
         cfg = self.cfg
         B, S, H = hidden_states.shape
         dev = hidden_states.device
@@ -191,16 +281,33 @@ class Qwen3MoeAttention(nn.Module):
         if max(L0) + S > cache.max_seq:
             raise ValueError("KV cache is full")
         x2d = hidden_states.reshape(B * S, H).to(torch.bfloat16).contiguous()
+        P = prefix.length if prefix is not None else 0
+        fresh = [l0 == 0 and n == 0 for l0, n in zip(L0, cache.dropped)]
+        if P and prefix.k is cache.k and prefix.slot < B:
+            raise ValueError("the prefix's slot is one of the batch's own")
+        if any(not f and p != P for f, p in zip(fresh, cache.prefix_len)):
+            raise ValueError("the cache was filled behind another prefix (or none)")
+        if attention_mask is not None and any(cache.dropped[:B]):
+            raise ValueError("attention_mask: the cache evicted rows (its paddings among them); pass no mask")
         pads = left_padding(attention_mask, B, S, L0)
-        if pads is not None:
-            for b in range(B):
-                cache.pad[b] = pads[b]
+        for b in range(B):
+            if pads is not None:
+                cache.pad[b] = cache.lead[b] = pads[b]
+            if fresh[b]:
+                # behind a prefix the distance to it counts, so paddings are left out of the positions
+                cache.prefix_len[b] = P
+                cache.offset[b] = P - cache.pad[b] if P else 0
         pad_now = cache.pad[:B]
-        pos = (torch.tensor(L0, dtype=torch.int32).unsqueeze(1) + torch.arange(S, dtype=torch.int32))
+        rows = (torch.tensor(L0, dtype=torch.int32).unsqueeze(1) + torch.arange(S, dtype=torch.int32))
+        pos = rows + torch.tensor(cache.offset[:B], dtype=torch.int32).unsqueeze(1)
+        # own rows apart from positions: behind a prefix, or in a cache that may evict
+        apart = P > 0 or cache.tracked
         if position_ids is not None:
             given = position_ids.reshape(B, S).to(torch.int32).cpu()
-            shifted = pos - torch.tensor(pad_now, dtype=torch.int32).unsqueeze(1)
-            real = shifted >= 0  # padding tokens may carry any position
+            shifted = pos - torch.tensor(cache.lead[:B], dtype=torch.int32).unsqueeze(1)
+            if P:
+                shifted = pos  # paddings are left out already
+            real = rows >= torch.tensor(pad_now, dtype=torch.int32).unsqueeze(1)  # padding tokens may carry any position
             if not (torch.equal(given, pos) or bool(torch.all((given == shifted) | ~real))):
                 raise ValueError("position_ids must continue each sequence's cache contiguously (or, with left "
                                  "padding, count from the first real token)")
@@ -208,23 +315,51 @@ class Qwen3MoeAttention(nn.Module):
         kv_start = (torch.tensor(pad_now, dtype=torch.int32).to(dev, non_blocking=True)
                     if any(pad_now) else None)
         slots = torch.arange(B, dtype=torch.int32).repeat_interleave(S).to(dev, non_blocking=True)
+        rows_dev = rows.reshape(-1).to(dev, non_blocking=True) if apart else None
         with stage(timer, "qkv_proj"):
             qkv = ops.linear(x2d, self.w.wqkv)
         with stage(timer, "qk_norm_rope"):
             q = ops.qk_norm_rope(qkv, positions, self.w.q_norm, self.w.k_norm, self.inv_freq,
                                  cfg.num_attention_heads, cfg.num_key_value_heads, cfg.rms_norm_eps,
-                                 cache.k, cache.v, cache_slot=slots)
+                                 cache.k, cache.v, cache_slot=slots, cache_rows=rows_dev, row_tokens=cache.tokens,
+                                 row_weights=cache.weights)
+        kp, vp, pslot = (prefix.k, prefix.v, prefix.slot) if P else (None, None, 0)
         if S == 1:
             kv_len = torch.tensor([l + 1 for l in L0], dtype=torch.int32).to(dev, non_blocking=True)
-            with stage(timer, "attention"):
-                attn = ops.attention_decode(q, cache.k, cache.v, kv_len, max(L0) + 1,
-                                            workspace=self._decode_ws, kv_start=kv_start)
+            if apart:
+                with stage(timer, "attention"):
+                    attn = ops.attention_prefix_decode(q, kp, vp, P, cache.k, cache.v, kv_len, max(L0) + 1,
+                                                       kv_start=kv_start, prefix_slot=pslot, weights=cache.weights)
+            else:
+                with stage(timer, "attention"):
+                    attn = ops.attention_decode(q, cache.k, cache.v, kv_len, max(L0) + 1,
+                                                workspace=self._decode_ws, kv_start=kv_start)
         else:
             q_start = torch.tensor(L0, dtype=torch.int32).to(dev, non_blocking=True)
             with stage(timer, "attention"):
-                attn = ops.attention_prefill(q, cache.k, cache.v, q_start, B, S, kv_start=kv_start)
+                if apart:
+                    attn = ops.attention_prefix_prefill(q, kp, vp, P, cache.k, cache.v, q_start, B, S,
+                                                        kv_start=kv_start, prefix_slot=pslot,
+                                                        return_lse=cache.tracked)
+                    if cache.tracked:
+                        attn, lse = attn
+                        self._score(q, lse, cache, q_start, B, S, kv_start, max(L0) + S)
+                else:
+                    attn = ops.attention_prefill(q, cache.k, cache.v, q_start, B, S, kv_start=kv_start)
         for b in range(B):
             cache.lengths[b] += S
         with stage(timer, "o_proj"):
             out = ops.linear(attn, self.w.wo)
         return out.reshape(B, S, H), cache
+
+    @staticmethod
+    def _score(q: torch.Tensor, lse: torch.Tensor, cache: KVCache, q_start: torch.Tensor, B: int, S: int,
+               kv_start: Optional[torch.Tensor], max_len: int) -> None:
+        """Add the attention weights of the call's last queries to the cache's."""
+        n = S if cache.score_queries is None else min(S, cache.score_queries)
+        if n < S:
+            nh, hd = q.shape[1:]
+            q = q.view(B, S, nh, hd)[:, S - n:].reshape(B * n, nh, hd)
+            lse = lse.view(B, S, nh)[:, S - n:].reshape(B * n, nh)
+            q_start = q_start + (S - n)
+        ops.attention_weights(q, lse, cache.k, q_start, B, n, cache.weights, kv_start=kv_start, max_len=max_len)

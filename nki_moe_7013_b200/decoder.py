@@ -73,7 +73,7 @@ class Qwen3MoeDecoderLayer(nn.Module):
         with stage(timer, "input_norm"):
             h = ops.rmsnorm(x2d, self.input_layernorm, eps)
         a, present = self.self_attn(h.reshape(B, S, H), position_ids, past_key_value, timer=timer,
-                                    attention_mask=attention_mask)
+                                    attention_mask=attention_mask, prefix=kwargs.get("prefix"))
         a2d = a.reshape(B * S, H)
         if getattr(self.mlp, "expert_parallel", False):
             with stage(timer, "post_norm"):

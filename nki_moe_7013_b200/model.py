@@ -19,6 +19,12 @@ on the device, so a whole step -- 48 layers of RMSNorm, QKV projection, QK
 norm + RoPE + cache append, split-KV decode attention, O projection, add &
 norm and the MoE block (one library call), then the final norm, the LM head and a greedy pick --
 captures into one CUDA graph and replays without the host.
+
+A prompt that many sequences share is run once, ``prefill_prefix``, and given
+to ``forward`` and ``DecodeSession`` as ``prefix``: one ``SharedPrefix`` per
+layer, read once per step for the whole batch.  A session with ``keep`` holds
+caches of bounded size: it evicts, in every layer, down to ``keep`` rows per
+KV head by accumulated attention weight whenever a cache is full.
 """
 from __future__ import annotations
 
@@ -27,7 +33,7 @@ from typing import List, Optional
 import torch
 
 from . import ops
-from .attention import KVCache
+from .attention import KVCache, SharedPrefix
 from .config import Qwen3MoeConfig
 from .decoder import Qwen3MoeDecoderLayer
 from .moe import MoEPlan, MoEWeights, WorkspacePool
@@ -129,23 +135,39 @@ class Qwen3MoeModel:
         m._share_workspace()
         return m
 
-    def new_caches(self, n_slots: int, max_seq: int) -> List[KVCache]:
-        return [layer.self_attn.new_cache(n_slots, max_seq) for layer in self.layers]
+    def new_caches(self, n_slots: int, max_seq: int, track: bool = False,
+                   score_queries: Optional[int] = None) -> List[KVCache]:
+        """One cache per layer; ``track`` / ``score_queries`` as in KVCache."""
+        return [layer.self_attn.new_cache(n_slots, max_seq, track=track, score_queries=score_queries)
+                for layer in self.layers]
+
+    def prefill_prefix(self, input_ids: torch.Tensor) -> List[SharedPrefix]:
+        """Run one prompt (P,) or (1, P) and return its rows in every layer as
+        a prefix that batches can share."""
+        ids = input_ids.reshape(1, -1)
+        caches = self.new_caches(1, ids.shape[1])
+        self.hidden_states(ids, caches)
+        return [c.as_prefix() for c in caches]
 
     def hidden_states(self, input_ids: torch.Tensor, past_key_values: Optional[List[KVCache]] = None,
-                      num_layers: Optional[int] = None, timer=None, moe_inputs: Optional[list] = None):
+                      num_layers: Optional[int] = None, timer=None, moe_inputs: Optional[list] = None,
+                      prefix: Optional[List[SharedPrefix]] = None):
         """input_ids (B, S) -> (hidden states (B, S, H) bf16 after the first
         ``num_layers`` layers (all by default), caches).  ``timer``: an
         ``attention.StageTimer`` given to every layer.  ``moe_inputs``: a
         list that receives each layer's MoE-block input (T, H) (layer-by-layer
-        parity checks: the routing each layer saw)."""
+        parity checks: the routing each layer saw).  ``prefix``: each layer's
+        shared prefix (``prefill_prefix``)."""
+        if prefix is not None and len(prefix) != len(self.layers):
+            raise ValueError(f"prefix holds {len(prefix)} layers for a model of {len(self.layers)}")
         B, S = input_ids.shape
         H = self.cfg.hidden_size
         caches = past_key_values if past_key_values is not None else self.new_caches(B, S)
         x = ops.embedding(input_ids.reshape(-1).to(torch.int32).contiguous(), self.embed).reshape(B, S, H)
         n = len(self.layers) if num_layers is None else num_layers
-        for layer, cache in zip(self.layers[:n], caches):
-            x = layer(x, past_key_value=cache, timer=timer, capture_intermediates=moe_inputs is not None)[0]
+        for l, (layer, cache) in enumerate(zip(self.layers[:n], caches)):
+            x = layer(x, past_key_value=cache, timer=timer, capture_intermediates=moe_inputs is not None,
+                      prefix=prefix[l] if prefix is not None else None)[0]
             if moe_inputs is not None:
                 moe_inputs.append(layer.last["moe_in"])
         return x, caches
@@ -164,13 +186,14 @@ class Qwen3MoeModel:
 
 
     def forward(self, input_ids: torch.Tensor, past_key_values: Optional[List[KVCache]] = None,
-                last_only: bool = False):
+                last_only: bool = False, prefix: Optional[List[SharedPrefix]] = None):
         """input_ids (B, S) -> (logits (B, S, V) bf16, caches); the eager path
         through the decoder-layer modules.  ``last_only``: logits of each
-        sequence's last position only, (B, 1, V)."""
+        sequence's last position only, (B, 1, V).  ``prefix``: each layer's
+        shared prefix, which the tokens follow."""
         B, S = input_ids.shape
         H = self.cfg.hidden_size
-        x, caches = self.hidden_states(input_ids, past_key_values)
+        x, caches = self.hidden_states(input_ids, past_key_values, prefix=prefix)
         if last_only:
             x = x[:, -1:].contiguous()
             S = 1
@@ -200,29 +223,52 @@ class DecodeSession:
     The caches hold ``context`` tokens per sequence on entry (config 2 fills
     them with ~N(0,1) values) and room for ``max_new`` more.  ``tokens`` (B,)
     int32 on the device is the input of the next step and is overwritten with
-    its greedy output; ``logits`` (B, V) bf16 holds the last step's logits."""
+    its greedy output; ``logits`` (B, V) bf16 holds the last step's logits.
+
+    ``prefix`` (``Qwen3MoeModel.prefill_prefix``): the sequences follow it; the
+    caches hold their own rows only.  ``keep`` / ``recent``: a session without
+    end -- when the caches are full (``context + max_new`` rows), ``step``
+    evicts them to ``keep`` rows per KV head, the ``recent`` newest tokens
+    among them, before it runs."""
 
     def __init__(self, model: Qwen3MoeModel, batch: int, context: int, max_new: int, seed: int = 0,
-                 fill_random: bool = True, split_k: bool = True):
+                 fill_random: bool = True, split_k: bool = True, prefix: Optional[List[SharedPrefix]] = None,
+                 keep: Optional[int] = None, recent: int = 0):
         cfg = model.cfg
         dev = model.device
         self.model = model
         self.B = batch
         self.max_seq = context + max_new
-        self.caches = model.new_caches(batch, self.max_seq)
+        if prefix is not None and len(prefix) != len(model.layers):
+            raise ValueError(f"prefix holds {len(prefix)} layers for a model of {len(model.layers)}")
+        if keep is not None and not (0 <= recent <= keep < self.max_seq):
+            raise ValueError("a session needs 0 <= recent <= keep < context + max_new")
+        self.prefix, self.keep, self.recent = prefix, keep, recent
+        P = prefix[0].length if prefix else 0
+        self.rows_used = context                                # rows of every cache in use (host)
+        self.caches = model.new_caches(batch, self.max_seq, track=keep is not None)
         if fill_random:
             for l, c in enumerate(self.caches):
                 c.fill_random(context, seed=seed * 100 + l)
+        for c in self.caches:
+            if c.tracked:  # the tokens of the rows the caches are entered with
+                c.tokens[:, :, :context] = torch.arange(P, P + context, dtype=torch.int32, device=dev)
         i32 = dict(dtype=torch.int32, device=dev)
-        self.positions = torch.full((batch,), context, **i32)   # position of the next token
-        self.kv_len = self.positions + 1                        # cache length once it is appended
+        self.positions = torch.full((batch,), P + context, **i32)  # position of the next token
+        self.kv_len = torch.full((batch,), context + 1, **i32)     # cache length once it is appended
+        # its cache row, where that is not its position
+        self.rows = torch.full((batch,), context, **i32) if (P or keep is not None) else None
         self.slots = torch.arange(batch, **i32)
         g = torch.Generator(device=dev)
         g.manual_seed(seed * 100 + 99)
         self.tokens = torch.randint(0, model.vocab_size, (batch,), generator=g, device=dev, dtype=torch.int32)
         self.plans = [MoEPlan(layer.mlp.weights, batch, cfg.num_experts_per_tok) for layer in model.layers]
-        lib_splits = ops._C.lib().qmoe_attention_decode_splits(batch, cfg.num_key_value_heads, self.max_seq)
-        ws = ops._C.lib().qmoe_attention_decode_workspace_size(batch, cfg.num_attention_heads, int(lib_splits))
+        if self.rows is not None:
+            ws = ops.attention_prefix_decode_workspace_size(batch, cfg.num_attention_heads, cfg.num_key_value_heads,
+                                                            P, self.max_seq, keep is not None)
+        else:
+            lib_splits = ops._C.lib().qmoe_attention_decode_splits(batch, cfg.num_key_value_heads, self.max_seq)
+            ws = ops._C.lib().qmoe_attention_decode_workspace_size(batch, cfg.num_attention_heads, int(lib_splits))
         self.attn_ws = torch.empty(max(int(ws), 1), dtype=torch.uint8, device=dev)
         # split-K scratch of the decode projections (one launch at a time uses it)
         self.split_ws = ops.gateup_split_workspace(dev) if (split_k and batch <= 16) else None
@@ -242,20 +288,39 @@ class DecodeSession:
         qkv = ops.linear(h, attn.w.wqkv, split_ws=self.split_ws)
         q = ops.qk_norm_rope(qkv, self.positions, attn.w.q_norm, attn.w.k_norm, attn.inv_freq,
                              cfg.num_attention_heads, cfg.num_key_value_heads, eps, cache.k, cache.v,
-                             cache_slot=self.slots)
-        a = ops.attention_decode(q, cache.k, cache.v, self.kv_len, self.max_seq, workspace=self.attn_ws)
+                             cache_slot=self.slots, cache_rows=self.rows, row_tokens=cache.tokens,
+                             row_weights=cache.weights)
+        if self.rows is not None:
+            px = self.prefix[l] if self.prefix else SharedPrefix(None, None, 0)
+            a = ops.attention_prefix_decode(q, px.k, px.v, px.length, cache.k, cache.v, self.kv_len, self.max_seq,
+                                            workspace=self.attn_ws, prefix_slot=px.slot, weights=cache.weights)
+        else:
+            a = ops.attention_decode(q, cache.k, cache.v, self.kv_len, self.max_seq, workspace=self.attn_ws)
         o = ops.linear(a, attn.w.wo, split_ws=self.split_ws)
         # add & norm + MoE + residual add, one library call
         self.plans[l].run_block(o, x, layer.post_attention_layernorm, eps, out)
 
     def step(self) -> torch.Tensor:
         """One decode step on the current stream (or the captured graph)."""
+        self._make_room()
         if self.graph is not None:
             self.graph.replay()
         else:
             self._step_kernels()
         self.steps_done += 1
+        self.rows_used += 1
         return self.tokens
+
+    def _make_room(self) -> None:
+        """Evict every layer's cache to ``keep`` rows when it is full."""
+        if self.keep is None or self.rows_used < self.max_seq:
+            return
+        for c in self.caches:
+            ops.kv_evict(c.k, c.v, c.weights, c.tokens, self.rows.clone(), self.max_seq, self.keep,
+                         recent=self.recent)
+        self.rows.fill_(self.keep)
+        self.kv_len.fill_(self.keep + 1)
+        self.rows_used = self.keep
 
     def _step_kernels(self) -> None:
         m = self.model
@@ -268,16 +333,20 @@ class DecodeSession:
         ops.linear(hf, m.lm_head, out=self.logits, split_ws=self.split_ws)
         # greedy pick + the next step's position and cache length, one launch
         ops.greedy_pick(self.logits, self.tokens, self.positions, self.kv_len)
+        if self.rows is not None:
+            self.rows.add_(1)
 
     def capture(self) -> None:
         """Capture one step into a CUDA graph (run one eager step first so
         every kernel's attributes are set outside the capture)."""
         dev = self.model.device
+        self._make_room()
         s = torch.cuda.Stream(dev)
         s.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(s):
             self._step_kernels()
             self.steps_done += 1
+            self.rows_used += 1
         torch.cuda.current_stream(dev).wait_stream(s)
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
