@@ -7,6 +7,7 @@ computes on the CPU.
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -32,6 +33,9 @@ def _stream(dev: torch.device):
 
 
 def _need(t: torch.Tensor, name: str, dtype=None, dim=None):
+    if (isinstance(t, torch.Tensor) and t.is_cuda and (dtype is None or t.dtype == dtype)
+            and (dim is None or t.dim() == dim) and t.is_contiguous()):
+        return t
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
     if t.device.type != "cuda":
@@ -634,10 +638,24 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 # shared prefixes and bounded caches
 # ----------------------------------------------------------------------------
 
+def _launch(dev: torch.device, what: str, fn, *args) -> None:
+    """fn(*args, stream) with ``dev`` current, on its current stream.  (The
+    device guard and the stream object cost 4 us of host time per call, which
+    a call of a few rows would wait for; both are skipped where they can be.)"""
+    i = dev.index
+    if torch._C._cuda_getDevice() == i:
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if st != 0:
+        _C.check(st, what)
+
+
 def _need_rows(t: torch.Tensor, name: str, dtype, k_cache: torch.Tensor):
     """A per-row array (n_slots, nkv, max_seq) of a cache."""
     _need(t, name, dtype, 3)
-    if tuple(t.shape) != tuple(k_cache.shape[:3]):
+    if t.shape != k_cache.shape[:3]:
         raise ValueError(f"{name} must be {tuple(k_cache.shape[:3])} like the cache's rows (got {tuple(t.shape)})")
     if t.device != k_cache.device:
         raise ValueError(f"{name} must be on the cache's device")
@@ -659,17 +677,17 @@ def _need_i32(t: Optional[torch.Tensor], name: str, n: int, dev):
         raise ValueError(f"{name} must hold {n} int32 on {dev}")
 
 
-def _need_prefix(k_prefix, v_prefix, prefix_len: int, prefix_slot: int, k_cache: torch.Tensor):
+def _need_prefix(k_prefix, v_prefix, prefix_len: int, k_cache: torch.Tensor):
     """(pointer, pointer, slots, rows per slot) of a prefix; nulls without one."""
     if prefix_len == 0:
         return None, None, 0, 0
     if k_prefix is None or v_prefix is None:
         raise ValueError("a prefix of more than 0 rows needs k_prefix and v_prefix")
     _need_cache(k_prefix, v_prefix, "prefix")
-    if k_prefix.shape[1] != k_cache.shape[1] or k_prefix.shape[3] != k_cache.shape[3] or \
-            k_prefix.device != k_cache.device:
+    n, nkv, rows, hd = k_prefix.shape
+    if nkv != k_cache.shape[1] or hd != k_cache.shape[3] or k_prefix.device != k_cache.device:
         raise ValueError("the prefix must have the cache's KV heads, head dim and device")
-    return _ptr(k_prefix), _ptr(v_prefix), k_prefix.shape[0], k_prefix.shape[2]
+    return k_prefix.data_ptr(), v_prefix.data_ptr(), n, rows
 
 
 def _need_heads(q: torch.Tensor, rows: int, k_cache: torch.Tensor):
@@ -682,6 +700,22 @@ def _need_heads(q: torch.Tensor, rows: int, k_cache: torch.Tensor):
 def _need_batch(B: int, cache_slot: Optional[torch.Tensor], k_cache: torch.Tensor):
     if cache_slot is None and B > k_cache.shape[0]:
         raise ValueError(f"{B} sequences in a cache of {k_cache.shape[0]} slots need cache_slot")
+
+
+@lru_cache(maxsize=256)
+def _prefix_decode_bytes(device: int, B: int, nh: int, nkv: int, prefix_len: int, max_len: int, weights: int) -> int:
+    with torch.cuda.device(device):
+        return int(_C.lib().qmoe_attention_prefix_decode_workspace_size(B, nh, nkv, prefix_len, max_len, weights))
+
+
+def _workspace(given: Optional[torch.Tensor], nbytes: int, dev) -> torch.Tensor:
+    if given is not None:
+        _need(given, "workspace", torch.uint8, 1)
+        if given.device != dev:
+            raise ValueError(f"workspace must be on {dev}")
+        if given.shape[0] >= nbytes:
+            return given
+    return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
 
 
 def attention_prefix_decode(q: torch.Tensor, k_prefix: Optional[torch.Tensor], v_prefix: Optional[torch.Tensor],
@@ -708,25 +742,20 @@ def attention_prefix_decode(q: torch.Tensor, k_prefix: Optional[torch.Tensor], v
     _need_i32(cache_slot, "cache_slot", B, dev)
     _need_i32(kv_start, "kv_start", B, dev)
     _need_batch(B, cache_slot, k_cache)
-    kp, vp, n_prefix, prefix_max = _need_prefix(k_prefix, v_prefix, prefix_len, prefix_slot, k_cache)
+    kp, vp, n_prefix, prefix_max = _need_prefix(k_prefix, v_prefix, prefix_len, k_cache)
     if weights is not None:
         _need_rows(weights, "weights", torch.float32, k_cache)
-    n_slots, nkv, max_seq = k_cache.shape[:3]
-    scale = hd ** -0.5 if scale is None else scale
-    lib = _C.lib()
+    n_slots, nkv, max_seq, _ = k_cache.shape
     out = torch.empty((B, nh * hd), dtype=torch.bfloat16, device=dev)
     if B == 0:
         return out
-    with torch.cuda.device(dev):
-        ws_bytes = int(lib.qmoe_attention_prefix_decode_workspace_size(B, nh, nkv, prefix_len, max_len,
-                                                                       0 if weights is None else 1))
-        if workspace is None or workspace.numel() < ws_bytes:
-            workspace = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
-        _C.check(lib.qmoe_attention_prefix_decode(
-            _ptr(q), kp, vp, n_prefix, prefix_max, prefix_slot, prefix_len, _ptr(k_cache), _ptr(v_cache),
-            _ptr(kv_len), _ptr(cache_slot), _ptr(kv_start), B, nh, nkv, hd, n_slots, max_seq, max_len, float(scale),
-            _ptr(weights), 1 if accumulate else 0, _ptr(out), _ptr(workspace), workspace.numel(), _stream(dev)),
-            "qmoe_attention_prefix_decode")
+    ws = _workspace(workspace, _prefix_decode_bytes(dev.index, B, nh, nkv, prefix_len, max_len,
+                                                    0 if weights is None else 1), dev)
+    _launch(dev, "qmoe_attention_prefix_decode", _C.lib().qmoe_attention_prefix_decode,
+            q.data_ptr(), kp, vp, n_prefix, prefix_max, prefix_slot, prefix_len, k_cache.data_ptr(),
+            v_cache.data_ptr(), kv_len.data_ptr(), _ptr(cache_slot), _ptr(kv_start), B, nh, nkv, hd, n_slots, max_seq,
+            max_len, hd ** -0.5 if scale is None else scale, _ptr(weights), 1 if accumulate else 0, out.data_ptr(),
+            ws.data_ptr(), ws.shape[0])
     return out
 
 
@@ -774,18 +803,15 @@ def attention_prefix_prefill(q: torch.Tensor, k_prefix: Optional[torch.Tensor], 
     _need_i32(cache_slot, "cache_slot", B, dev)
     _need_i32(kv_start, "kv_start", B, dev)
     _need_batch(B, cache_slot, k_cache)
-    kp, vp, n_prefix, prefix_max = _need_prefix(k_prefix, v_prefix, prefix_len, prefix_slot, k_cache)
-    n_slots, nkv, max_seq = k_cache.shape[:3]
-    scale = hd ** -0.5 if scale is None else scale
+    kp, vp, n_prefix, prefix_max = _need_prefix(k_prefix, v_prefix, prefix_len, k_cache)
+    n_slots, nkv, max_seq, _ = k_cache.shape
     out = torch.empty((B * S, nh * hd), dtype=torch.bfloat16, device=dev)
     lse = torch.empty((B * S, nh), dtype=torch.float32, device=dev) if return_lse else None
-    if B * S == 0:
-        return (out, lse) if return_lse else out
-    with torch.cuda.device(dev):
-        _C.check(_C.lib().qmoe_attention_prefix_prefill(
-            _ptr(q), kp, vp, n_prefix, prefix_max, prefix_slot, prefix_len, _ptr(k_cache), _ptr(v_cache),
-            _ptr(q_start), _ptr(cache_slot), _ptr(kv_start), B, S, nh, nkv, hd, n_slots, max_seq, float(scale),
-            _ptr(out), _ptr(lse), _stream(dev)), "qmoe_attention_prefix_prefill")
+    if B * S > 0:
+        _launch(dev, "qmoe_attention_prefix_prefill", _C.lib().qmoe_attention_prefix_prefill,
+                q.data_ptr(), kp, vp, n_prefix, prefix_max, prefix_slot, prefix_len, k_cache.data_ptr(),
+                v_cache.data_ptr(), q_start.data_ptr(), _ptr(cache_slot), _ptr(kv_start), B, S, nh, nkv, hd, n_slots,
+                max_seq, hd ** -0.5 if scale is None else scale, out.data_ptr(), _ptr(lse))
     return (out, lse) if return_lse else out
 
 
@@ -813,15 +839,12 @@ def attention_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor,
     _need_i32(kv_start, "kv_start", B, dev)
     _need_batch(B, cache_slot, k_cache)
     _need_rows(weights, "weights", torch.float32, k_cache)
-    n_slots, nkv, max_seq = k_cache.shape[:3]
-    scale = hd ** -0.5 if scale is None else scale
-    if B * S == 0:
-        return weights
-    with torch.cuda.device(dev):
-        _C.check(_C.lib().qmoe_attention_weights(
-            _ptr(q), _ptr(lse), _ptr(k_cache), _ptr(q_start), _ptr(cache_slot), _ptr(kv_start), B, S, nh, nkv, hd,
-            n_slots, max_seq, max_seq if max_len is None else max_len, float(scale), _ptr(weights),
-            1 if accumulate else 0, _stream(dev)), "qmoe_attention_weights")
+    n_slots, nkv, max_seq, _ = k_cache.shape
+    if B * S > 0:
+        _launch(dev, "qmoe_attention_weights", _C.lib().qmoe_attention_weights,
+                q.data_ptr(), lse.data_ptr(), k_cache.data_ptr(), q_start.data_ptr(), _ptr(cache_slot),
+                _ptr(kv_start), B, S, nh, nkv, hd, n_slots, max_seq, max_seq if max_len is None else max_len,
+                hd ** -0.5 if scale is None else scale, weights.data_ptr(), 1 if accumulate else 0)
     return weights
 
 
@@ -850,15 +873,13 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor
     n_slots, nkv, max_seq, hd = k_cache.shape
     if B == 0:
         return
-    lib = _C.lib()
-    ws_bytes = int(lib.qmoe_kv_evict_workspace_size(B, nkv, max_len, keep))
-    if workspace is None or workspace.numel() < ws_bytes:
-        workspace = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        _C.check(lib.qmoe_kv_evict(
-            _ptr(k_cache), _ptr(v_cache), _ptr(weights), _ptr(tokens), _ptr(kv_len), _ptr(cache_slot),
-            _ptr(kv_start), B, nkv, hd, n_slots, max_seq, max_len, keep, recent, _ptr(workspace),
-            workspace.numel(), _stream(dev)), "qmoe_kv_evict")
+    # a count, the new length, and a source and a destination per move, for every KV head
+    nbytes = B * nkv * (2 + 2 * max(0, min(keep, max_len))) * 4
+    ws = _workspace(workspace, nbytes, dev)
+    _launch(dev, "qmoe_kv_evict", _C.lib().qmoe_kv_evict,
+            k_cache.data_ptr(), v_cache.data_ptr(), weights.data_ptr(), tokens.data_ptr(), kv_len.data_ptr(),
+            _ptr(cache_slot), _ptr(kv_start), B, nkv, hd, n_slots, max_seq, max_len, keep, recent, ws.data_ptr(),
+            ws.shape[0])
 
 
 # ----------------------------------------------------------------------------
