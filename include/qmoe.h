@@ -507,10 +507,13 @@ QMOE_API int qmoe_attention_prefix_prefill(const void* q, const void* k_prefix, 
                                            const int32_t* kv_start, int64_t B, int64_t S, int64_t nh, int64_t nkv,
                                            int64_t head_dim, int64_t n_slots, int64_t max_seq, float scale,
                                            void* out, float* lse, void* stream);
+QMOE_API size_t qmoe_attention_weights_workspace_size(int64_t B, int64_t S, int64_t nh, int64_t nkv,
+                                                      int64_t max_len);
 QMOE_API int qmoe_attention_weights(const void* q, const float* lse, const void* k_cache, const int32_t* q_start,
                                     const int32_t* cache_slot, const int32_t* kv_start, int64_t B, int64_t S,
                                     int64_t nh, int64_t nkv, int64_t head_dim, int64_t n_slots, int64_t max_seq,
-                                    int64_t max_len, float scale, float* weights, int accumulate, void* stream);
+                                    int64_t max_len, float scale, float* weights, int accumulate, void* workspace,
+                                    size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
  * Eviction from a cache by accumulated attention weight (no counterpart in

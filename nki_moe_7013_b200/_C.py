@@ -66,8 +66,9 @@ _SIGNATURES = {
                                            I64, ctypes.c_float, P, I32, P, P, SZ, P]),
     "qmoe_attention_prefix_prefill": (I32, [P, P, P, I64, I64, I64, I64, P, P, P, P, P, I64, I64, I64, I64, I64,
                                             I64, I64, ctypes.c_float, P, P, P]),
+    "qmoe_attention_weights_workspace_size": (SZ, [I64, I64, I64, I64, I64]),
     "qmoe_attention_weights": (I32, [P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, ctypes.c_float, P,
-                                     I32, P]),
+                                     I32, P, SZ, P]),
     "qmoe_kv_evict_workspace_size": (SZ, [I64, I64, I64, I64]),
     "qmoe_kv_evict": (I32, [P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, P, SZ, P]),
     "qmoe_routing_histogram": (I32, [P, I64, I64, I64, P, P]),

@@ -64,6 +64,31 @@ __device__ __forceinline__ bool own_range(const int32_t* kv_len, const int32_t* 
   return ok;
 }
 
+// One lane of a converged warp, chosen so that the compiler knows it is one: a
+// role that issues MMAs under it keeps their descriptors in uniform registers.
+// (Under lane == 0 every tcgen05.mma is wrapped in a loop over the lanes and
+// takes 120 cycles to issue, whatever its size; under this one 16.)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
+// D (+)= A B^T over K = 128: eight MMAs on two swizzled 32 KB tiles, the
+// descriptors' offsets known at compile time.
+template <bool kAdd = false>
+__device__ __forceinline__ void umma_bf16_k128(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc) {
+#pragma unroll
+  for (int kk = 0; kk < kFaD / 16; ++kk) {
+    const uint32_t off = ((kk >> 2) * kFaHalfBytes + (kk & 3) * 32) >> 4;
+    umma_bf16(d, adesc + off, bdesc + off, idesc, kAdd || kk > 0 ? 1u : 0u);
+  }
+}
+
 // One 16-byte chunk of a 128-byte-swizzled 64-column half tile.
 __device__ __forceinline__ uint32_t sw128_addr(uint32_t tile, int row, int chunk) {
   return tile + uint32_t(chunk >> 3) * kSdHalfBytes + uint32_t(row) * 128u + (uint32_t((chunk ^ row) & 7) << 4);

@@ -963,6 +963,27 @@ SharedDecodePlan shared_decode_plan(int64_t B, int64_t G, int64_t nkv, int64_t P
   return p;
 }
 
+// How the queries that score a cache are cut: blocks of 512 rows, each
+// against chunks of `chunk` query tiles.
+struct AttnWeightsPlan {
+  int64_t key_blocks, chunks, chunk;
+};
+
+AttnWeightsPlan attn_weights_plan(int64_t B, int64_t S, int64_t G, int64_t nkv, int64_t max_len) {
+  AttnWeightsPlan p{};
+  const int64_t sms = std::max(1, num_sms(0));
+  const int64_t q_tiles = (S + qmoe::kFaRows / G - 1) / (qmoe::kFaRows / G);
+  p.key_blocks = (max_len + qmoe::kAwKeys - 1) / qmoe::kAwKeys;
+  // eight units per SM where there are so many (a causal prompt's units differ
+  // in length), each of eight query tiles or more (its K tiles are as large as
+  // four)
+  const int64_t base = p.key_blocks * B * nkv;
+  const int64_t want = std::max<int64_t>(1, std::min((8 * sms + base - 1) / base, q_tiles / 8));
+  p.chunk = (q_tiles + want - 1) / want;
+  p.chunks = (q_tiles + p.chunk - 1) / p.chunk;
+  return p;
+}
+
 int check_shared_attention(const char* what, int64_t head_dim, int64_t nh, int64_t nkv, int64_t n_slots,
                            int64_t max_seq, float scale) {
   QMOE_REQUIRE(head_dim == qmoe::kAttnD, QMOE_ERR_UNSUPPORTED_SHAPE, "%s: head_dim must be 128", what);
@@ -1710,24 +1731,35 @@ int qmoe_attention_prefix_prefill(const void* q, const void* k_prefix, const voi
                        tk, tv, tkp, tvp, a);
 }
 
+size_t qmoe_attention_weights_workspace_size(int64_t B, int64_t S, int64_t nh, int64_t nkv, int64_t max_len) {
+  if (B <= 0 || S <= 0 || nkv <= 0 || nh <= 0 || nh % nkv != 0 || max_len <= 0) return 0;
+  const AttnWeightsPlan p = attn_weights_plan(B, S, nh / nkv, nkv, max_len);
+  return p.chunks > 1 ? size_t(p.chunks * B * nkv * p.key_blocks) * qmoe::kAwKeys * sizeof(float) : 0;
+}
+
 int qmoe_attention_weights(const void* q, const float* lse, const void* k_cache, const int32_t* q_start,
                            const int32_t* cache_slot, const int32_t* kv_start, int64_t B, int64_t S, int64_t nh,
                            int64_t nkv, int64_t head_dim, int64_t n_slots, int64_t max_seq, int64_t max_len,
-                           float scale, float* weights, int accumulate, void* stream) {
+                           float scale, float* weights, int accumulate, void* workspace, size_t workspace_bytes,
+                           void* stream) {
   QMOE_REQUIRE(q && lse && k_cache && q_start && weights, QMOE_ERR_INVALID_ARGUMENT,
                "attention_weights: null pointer");
   QMOE_CHECK(check_shared_attention("attention_weights", head_dim, nh, nkv, n_slots, max_seq, scale));
-  QMOE_REQUIRE(B >= 0 && B <= 65535 && S >= 0 && S <= max_len && max_len <= max_seq && (cache_slot || B <= n_slots),
+  QMOE_REQUIRE(B >= 0 && B * nkv <= 65535 && S >= 0 && S <= max_len && max_len <= max_seq &&
+                   (cache_slot || B <= n_slots),
                QMOE_ERR_INVALID_ARGUMENT, "attention_weights: bad sizes");
-  const int64_t blocks = (max_len + qmoe::kFaRows - 1) / qmoe::kFaRows * nkv * B;
-  QMOE_REQUIRE(B * S < (int64_t(1) << 30) && blocks < (int64_t(1) << 31), QMOE_ERR_INVALID_ARGUMENT,
-               "attention_weights: too many queries");
-  QMOE_REQUIRE(aligned16(q) && aligned16(k_cache), QMOE_ERR_MISALIGNED,
+  QMOE_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(workspace), QMOE_ERR_MISALIGNED,
                "attention_weights: pointers must be 16-byte aligned");
   DeviceInfo* d = nullptr;
   QMOE_CHECK(device_info(&d));
   if (B == 0 || S == 0) return QMOE_OK;
   const int64_t G = nh / nkv;
+  const AttnWeightsPlan p = attn_weights_plan(B, S, G, nkv, max_len);
+  const int64_t units = p.chunks * B * nkv * p.key_blocks;
+  QMOE_REQUIRE(B * S < (int64_t(1) << 30) && units < (int64_t(1) << 30), QMOE_ERR_INVALID_ARGUMENT,
+               "attention_weights: too many queries");
+  QMOE_REQUIRE(workspace_bytes >= qmoe_attention_weights_workspace_size(B, S, nh, nkv, max_len),
+               QMOE_ERR_WORKSPACE_TOO_SMALL, "attention_weights: workspace too small");
   CUtensorMap tq, tk;
   QMOE_CHECK(make_tmap_bf16_3d(&tq, q, 128, uint64_t(nh), uint64_t(B * S), 256, uint64_t(nh) * 256, 64, uint32_t(G),
                                uint32_t(qmoe::kFaRows / G)));
@@ -1738,6 +1770,7 @@ int qmoe_attention_weights(const void* q, const float* lse, const void* k_cache,
   a.cache_slot = cache_slot;
   a.kv_start = kv_start;
   a.weights = weights;
+  a.partial = p.chunks > 1 ? static_cast<float*>(workspace) : nullptr;
   a.B = int(B);
   a.S = int(S);
   a.nh = int(nh);
@@ -1747,11 +1780,18 @@ int qmoe_attention_weights(const void* q, const float* lse, const void* k_cache,
   a.max_seq = int(max_seq);
   a.max_len = int(max_len);
   a.accumulate = accumulate ? 1 : 0;
+  a.key_blocks = int(p.key_blocks);
+  a.n_chunks = int(p.chunks);
+  a.chunk = int(p.chunk);
   a.scale_log2 = scale * 1.4426950408889634f;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
   QMOE_CHECK(set_smem(qmoe::attn_weights_kernel, qmoe::kAwSmemBytes));
-  return launch_kernel(qmoe::attn_weights_kernel, dim3(unsigned(blocks)), dim3(qmoe::kAwThreads),
-                       size_t(qmoe::kAwSmemBytes), static_cast<cudaStream_t>(stream), true, "attn_weights_kernel", tq,
-                       tk, a);
+  QMOE_CHECK(launch_kernel(qmoe::attn_weights_kernel, dim3(unsigned(std::min<int64_t>(units, d->sms))),
+                           dim3(qmoe::kAwThreads), size_t(qmoe::kAwSmemBytes), s, true, "attn_weights_kernel", tq, tk,
+                           a));
+  if (p.chunks == 1) return QMOE_OK;
+  return launch_kernel(qmoe::attn_weights_join_kernel, dim3(unsigned(p.key_blocks * qmoe::kAwTiles), unsigned(B * nkv)),
+                       dim3(qmoe::kFaRows), 0, s, true, "attn_weights_join_kernel", a);
 }
 
 size_t qmoe_kv_evict_workspace_size(int64_t B, int64_t nkv, int64_t max_len, int64_t keep) {

@@ -708,6 +708,12 @@ def _prefix_decode_bytes(device: int, B: int, nh: int, nkv: int, prefix_len: int
         return int(_C.lib().qmoe_attention_prefix_decode_workspace_size(B, nh, nkv, prefix_len, max_len, weights))
 
 
+@lru_cache(maxsize=256)
+def _weights_bytes(device: int, B: int, S: int, nh: int, nkv: int, max_len: int) -> int:
+    with torch.cuda.device(device):
+        return int(_C.lib().qmoe_attention_weights_workspace_size(B, S, nh, nkv, max_len))
+
+
 def _workspace(given: Optional[torch.Tensor], nbytes: int, dev) -> torch.Tensor:
     if given is not None:
         _need(given, "workspace", torch.uint8, 1)
@@ -818,7 +824,7 @@ def attention_prefix_prefill(q: torch.Tensor, k_prefix: Optional[torch.Tensor], 
 def attention_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, q_start: torch.Tensor, B: int, S: int,
                       weights: torch.Tensor, accumulate: bool = True, scale: Optional[float] = None,
                       cache_slot: Optional[torch.Tensor] = None, kv_start: Optional[torch.Tensor] = None,
-                      max_len: Optional[int] = None) -> torch.Tensor:
+                      max_len: Optional[int] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention weights of S queries per sequence, summed per own cache row:
     ``weights`` (n_slots, nkv, max_seq) fp32 += (``accumulate=False``: =) the
     sum over the queries and the KV head's query heads of exp(scale q.k - lse).
@@ -841,10 +847,13 @@ def attention_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor,
     _need_rows(weights, "weights", torch.float32, k_cache)
     n_slots, nkv, max_seq, _ = k_cache.shape
     if B * S > 0:
+        max_len = max_seq if max_len is None else max_len
+        ws = _workspace(workspace, _weights_bytes(dev.index, B, S, nh, nkv, max_len), dev)
         _launch(dev, "qmoe_attention_weights", _C.lib().qmoe_attention_weights,
                 q.data_ptr(), lse.data_ptr(), k_cache.data_ptr(), q_start.data_ptr(), _ptr(cache_slot),
-                _ptr(kv_start), B, S, nh, nkv, hd, n_slots, max_seq, max_seq if max_len is None else max_len,
-                hd ** -0.5 if scale is None else scale, weights.data_ptr(), 1 if accumulate else 0)
+                _ptr(kv_start), B, S, nh, nkv, hd, n_slots, max_seq, max_len,
+                hd ** -0.5 if scale is None else scale, weights.data_ptr(), 1 if accumulate else 0, ws.data_ptr(),
+                ws.shape[0])
     return weights
 
 

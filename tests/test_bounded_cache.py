@@ -121,9 +121,9 @@ def test_prefill_and_weights_refusals(lib, p):
                    (dict(B=3), -1), (dict(scale=0.0), -1), (dict(out=p + 4), -3), (dict(kp=p + 8), -3)):
         assert prefill(**kw) == st, kw
 
-    def weights(q=p, lse=p, k=p, w=p, B=2, S=4, nh=32, nkv=4, hd=128, max_seq=64, max_len=64, scale=0.1):
+    def weights(q=p, lse=p, k=p, w=p, B=2, S=4, nh=32, nkv=4, hd=128, max_seq=64, max_len=64, scale=0.1, size=1 << 30):
         return lib.qmoe_attention_weights(q, lse, k, p, None, None, B, S, nh, nkv, hd, 2, max_seq, max_len, f(scale),
-                                          w, 1, None)
+                                          w, 1, p, size, None)
 
     for kw, st in ((dict(q=None), -1), (dict(lse=None), -1), (dict(w=None), -1), (dict(S=65), -1),
                    (dict(max_len=65), -1), (dict(max_len=3), -1), (dict(hd=64), -2), (dict(nh=6), -1),
