@@ -212,34 +212,27 @@ __global__ void __launch_bounds__(kFaThreads, 1)
     }
   } else if (warp == 9) {
     // ---------------- MMA issuer ----------------
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t idesc_s = make_idesc_bf16(kFaRows, kFaRows);
       const uint32_t idesc_o = make_idesc_bf16(kFaRows, kFaD) | (1u << 16);  // B (V) MN-major
-      const uint32_t q_addr = smem_u32(sQ), p_addr = smem_u32(sP), pool = smem_u32(sPool);
+      const uint64_t q_desc = make_sw128_desc(smem_u32(sQ)), p_desc = make_sw128_desc(smem_u32(sP));
+      const uint64_t k_desc = make_sw128_desc(smem_u32(sPool));
+      const uint64_t v_desc = make_sw128_desc_mn(smem_u32(sPool), kFaHalfBytes, 1024);
+      constexpr uint32_t kTile = kFaTileBytes >> 4;
       auto item_full = [&](int n) {
         return fa_wait(&full[n % kFaPool], (n / kFaPool) & 1, abort_flag, kDevErrWaitTimeoutMma);
       };
       auto issue_s = [&](int g, int i) {  // S_g = Q_g K_i^T
-        const uint32_t k_addr = pool + ((2 * i) % kFaPool) * kFaTileBytes;
-        const uint32_t qa = q_addr + g * kFaTileBytes;
-        const uint32_t d = tmem_base + g * kFaRows;
-#pragma unroll
-        for (int kk = 0; kk < kFaD / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kFaHalfBytes + (kk & 3) * 32;
-          umma_bf16(d, make_sw128_desc(qa + off), make_sw128_desc(k_addr + off), idesc_s, kk > 0 ? 1u : 0u);
-        }
+        umma_bf16_k128(tmem_base + g * kFaRows, q_desc + g * kTile, k_desc + ((2 * i) % kFaPool) * kTile, idesc_s);
         umma_commit(&s_full[g]);
       };
       auto issue_pv = [&](int g, int i) {  // O_g (+)= P_g V_i
-        const uint32_t v_addr = pool + ((2 * i + 1) % kFaPool) * kFaTileBytes;
-        const uint32_t pa = p_addr + g * kFaTileBytes;
+        const uint64_t vd = v_desc + ((2 * i + 1) % kFaPool) * kTile, pd = p_desc + g * kTile;
         const uint32_t d = tmem_base + 2 * kFaRows + g * kFaD;
 #pragma unroll
-        for (int kk = 0; kk < kFaRows / 16; ++kk) {  // 16 keys per MMA
-          const uint64_t adesc = make_sw128_desc(pa + (kk >> 2) * kFaHalfBytes + (kk & 3) * 32);
-          const uint64_t bdesc = make_sw128_desc_mn(v_addr + kk * 16 * 128, kFaHalfBytes, 1024);
-          umma_bf16(d, adesc, bdesc, idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
-        }
+        for (int kk = 0; kk < kFaRows / 16; ++kk)  // 16 keys per MMA
+          umma_bf16(d, pd + (((kk >> 2) * kFaHalfBytes + (kk & 3) * 32) >> 4), vd + ((kk * 16 * 128) >> 4), idesc_o,
+                    (i > 0 || kk > 0) ? 1u : 0u);
       };
       bool ok = fa_wait(q_full, 0, abort_flag, kDevErrWaitTimeoutMma) && item_full(0);
       if (ok) {
