@@ -925,10 +925,31 @@ int make_tmap_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t str
                            uint32_t(box_rows), 1);
 }
 
+// flash_prefix_kernel with its four forms behind one call.
+int launch_flash_prefix(bool partial, bool split, int64_t ctas, const CUtensorMap& tq, const CUtensorMap& tk,
+                        const CUtensorMap& tv, const CUtensorMap& tkp, const CUtensorMap& tvp,
+                        const qmoe::FlashPrefixArgs& a, cudaStream_t s) {
+  auto* kernel = partial ? (split ? qmoe::flash_prefix_kernel<true, true> : qmoe::flash_prefix_kernel<true, false>)
+                         : (split ? qmoe::flash_prefix_kernel<false, true> : qmoe::flash_prefix_kernel<false, false>);
+  QMOE_CHECK(set_smem(kernel, qmoe::kFpSmemBytes));
+  return launch_kernel(kernel, dim3(unsigned(ctas)), dim3(qmoe::kFaThreads), size_t(qmoe::kFpSmemBytes), s, true,
+                       "flash_prefix_kernel", tq, tk, tv, tkp, tvp, a);
+}
+
+// Row tiles of flash_prefix_kernel: a CTA takes two that share its key tiles,
+// or splits the key tiles of one between its two groups.  Splitting halves a
+// CTA's steps (and joins the halves, about a step's time) for twice the CTAs,
+// so it pays while they still run in as many waves (one CTA per SM).
+bool flash_prefix_split(int64_t row_tiles, int64_t columns, double key_tiles, int64_t sms) {
+  const int64_t pair_waves = ((row_tiles + 1) / 2 * columns + sms - 1) / sms;
+  const int64_t split_waves = (row_tiles * columns + sms - 1) / sms;
+  return double(split_waves) * (key_tiles / 2 + 1) < double(pair_waves) * key_tiles;
+}
+
 // How a decode step over a shared prefix is cut into parts.
 struct SharedDecodePlan {
-  bool tc;             // the prefix part runs on the tcgen05 kernel
-  int64_t row_tiles;   // 16-row tiles, or 256-row pairs of tiles, of one KV head's rows
+  bool tc, split;      // the prefix part runs on the tcgen05 kernel, and splits its key tiles
+  int64_t row_tiles;   // 16-row tiles, or the tcgen05 kernel's row blocks, of one KV head's rows
   int64_t psplits, pchunk, osplits;
 };
 
@@ -942,14 +963,23 @@ SharedDecodePlan shared_decode_plan(int64_t B, int64_t G, int64_t nkv, int64_t P
   const int64_t rows = B * G;
   p.tc = P > 0 && rows > kPrefixMmaRows;
   if (p.tc) {
-    // one CTA per SM
-    const int64_t pair_rows = 2 * (qmoe::kFaRows / G * G);
-    p.row_tiles = (rows + pair_rows - 1) / pair_rows;
-    const int64_t tiles = (P + qmoe::kFaRows - 1) / qmoe::kFaRows;
-    const int64_t want = std::max<int64_t>(1, std::min(tiles, sms / (p.row_tiles * nkv)));
-    const int64_t per_part = (tiles + want - 1) / want;
-    p.pchunk = per_part * qmoe::kFaRows;
-    p.psplits = (tiles + per_part - 1) / per_part;
+    // one CTA per SM; the split form where it leaves a CTA fewer steps
+    const int64_t per_tile = qmoe::kFaRows / G, tiles = (P + qmoe::kFaRows - 1) / qmoe::kFaRows;
+    const int64_t row_tiles = (B + per_tile - 1) / per_tile;
+    double best = 0;
+    for (int split = 0; split < 2; ++split) {
+      const int64_t blocks = split ? row_tiles : (row_tiles + 1) / 2;
+      const int64_t want = std::max<int64_t>(1, std::min(tiles, sms / (blocks * nkv)));
+      const int64_t per_part = (tiles + want - 1) / want, parts = (tiles + per_part - 1) / per_part;
+      const double waves = double((blocks * nkv * parts + sms - 1) / sms);
+      const double cost = waves * (split ? double((per_part + 1) / 2 + 1) : double(per_part));
+      if (split && cost >= best) break;
+      best = cost;
+      p.split = split != 0;
+      p.row_tiles = blocks;
+      p.pchunk = per_part * qmoe::kFaRows;
+      p.psplits = parts;
+    }
   } else if (P > 0) {
     // two CTAs per SM, parts of at least 128 keys
     p.row_tiles = (rows + 15) / 16;
@@ -1604,17 +1634,14 @@ int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void
     fa.nh = int(nh);
     fa.nkv = int(nkv);
     fa.B = int(B);
-    fa.n_pairs = int(p.row_tiles);
+    fa.n_blocks = int(p.row_tiles);
     fa.P = int(prefix_len);
     fa.prefix_z = int(prefix_slot * nkv);
     fa.G = int(G);
     fa.nparts = int(nparts);
     fa.tiles_per_part = int(p.pchunk / qmoe::kFaRows);
     fa.scale_log2 = scale * 1.4426950408889634f;
-    QMOE_CHECK(set_smem(qmoe::flash_prefix_kernel<true>, qmoe::kFaSmemBytes));
-    QMOE_CHECK(launch_kernel(qmoe::flash_prefix_kernel<true>, dim3(unsigned(p.row_tiles * nkv * p.psplits)),
-                             dim3(qmoe::kFaThreads), size_t(qmoe::kFaSmemBytes), s, true, "flash_prefix_kernel", tq,
-                             tk128, tv128, tk128, tv128, fa));
+    QMOE_CHECK(launch_flash_prefix(true, p.split, p.row_tiles * nkv * p.psplits, tq, tk128, tv128, tk128, tv128, fa, s));
   } else if (prefix_len > 0) {
     QMOE_CHECK(make_tmap_rows(&tkp, k_prefix, prefix_len, prefix_max, n_prefix_slots * nkv, qmoe::kSdKeys));
     QMOE_CHECK(make_tmap_rows(&tvp, v_prefix, prefix_len, prefix_max, n_prefix_slots * nkv, qmoe::kSdKeys));
@@ -1687,10 +1714,11 @@ int qmoe_attention_prefix_prefill(const void* q, const void* k_prefix, const voi
   QMOE_CHECK(check_shared_attention("attention_prefix_prefill", head_dim, nh, nkv, n_slots, max_seq, scale));
   QMOE_CHECK(check_prefix("attention_prefix_prefill", k_prefix, v_prefix, n_prefix_slots, prefix_max, prefix_slot,
                           prefix_len, nkv));
-  const int64_t n_pairs = (S + 2 * qmoe::kFaRows - 1) / (2 * qmoe::kFaRows);
   QMOE_REQUIRE(B >= 0 && B <= 65535 && S >= 0 && S <= max_seq && (cache_slot || B <= n_slots),
                QMOE_ERR_INVALID_ARGUMENT, "attention_prefix_prefill: bad sizes");
-  QMOE_REQUIRE(B * S < (int64_t(1) << 30) && n_pairs * nh * B < (int64_t(1) << 31), QMOE_ERR_INVALID_ARGUMENT,
+  const int64_t G = nh / nkv, per_tile = qmoe::kFaRows / G;
+  const int64_t row_tiles = (S + per_tile - 1) / per_tile;  // of one (sequence, KV head)
+  QMOE_REQUIRE(B * S < (int64_t(1) << 30) && row_tiles * nkv * B < (int64_t(1) << 31), QMOE_ERR_INVALID_ARGUMENT,
                "attention_prefix_prefill: too many queries");
   QMOE_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out), QMOE_ERR_MISALIGNED,
                "attention_prefix_prefill: pointers must be 16-byte aligned");
@@ -1698,8 +1726,8 @@ int qmoe_attention_prefix_prefill(const void* q, const void* k_prefix, const voi
   QMOE_CHECK(device_info(&d));
   if (B == 0 || S == 0) return QMOE_OK;
   CUtensorMap tq, tk, tv, tkp, tvp;
-  QMOE_CHECK(make_tmap_bf16_3d(&tq, q, 128, uint64_t(nh), uint64_t(B * S), 256, uint64_t(nh) * 256, 64, 1,
-                               qmoe::kFaRows));
+  QMOE_CHECK(make_tmap_bf16_3d(&tq, q, 128, uint64_t(nh), uint64_t(B * S), 256, uint64_t(nh) * 256, 64, uint32_t(G),
+                               uint32_t(per_tile)));
   QMOE_CHECK(make_tmap_rows(&tk, k_cache, max_seq, max_seq, n_slots * nkv, qmoe::kFaRows));
   QMOE_CHECK(make_tmap_rows(&tv, v_cache, max_seq, max_seq, n_slots * nkv, qmoe::kFaRows));
   tkp = tk;
@@ -1720,15 +1748,14 @@ int qmoe_attention_prefix_prefill(const void* q, const void* k_prefix, const voi
   a.max_seq = int(max_seq);
   a.n_slots = int(n_slots);
   a.B = int(B);
-  a.n_pairs = int(n_pairs);
+  const bool split = flash_prefix_split(row_tiles, nkv * B, double(prefix_len + S) / qmoe::kFaRows, d->sms);
+  a.n_blocks = int(split ? row_tiles : (row_tiles + 1) / 2);
   a.P = int(prefix_len);
   a.prefix_z = int(prefix_slot * nkv);
-  a.G = int(nh / nkv);
+  a.G = int(G);
   a.scale_log2 = scale * 1.4426950408889634f;
-  QMOE_CHECK(set_smem(qmoe::flash_prefix_kernel<false>, qmoe::kFaSmemBytes));
-  return launch_kernel(qmoe::flash_prefix_kernel<false>, dim3(unsigned(n_pairs * nh * B)), dim3(qmoe::kFaThreads),
-                       size_t(qmoe::kFaSmemBytes), static_cast<cudaStream_t>(stream), true, "flash_prefix_kernel", tq,
-                       tk, tv, tkp, tvp, a);
+  return launch_flash_prefix(false, split, a.n_blocks * nkv * B, tq, tk, tv, tkp, tvp, a,
+                             static_cast<cudaStream_t>(stream));
 }
 
 size_t qmoe_attention_weights_workspace_size(int64_t B, int64_t S, int64_t nh, int64_t nkv, int64_t max_len) {
