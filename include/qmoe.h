@@ -488,8 +488,6 @@ QMOE_API int qmoe_attention_decode(const void* q, const void* k_cache, const voi
  *   of their rows (of qmoe_attention_prefix_prefill; the prefix's share stays
  *   in it).  max_len bounds q_start + S.
  * ---------------------------------------------------------------------- */
-QMOE_API int64_t qmoe_attention_prefix_decode_parts(int64_t B, int64_t nh, int64_t nkv, int64_t prefix_len,
-                                                    int64_t max_len);
 QMOE_API size_t qmoe_attention_prefix_decode_workspace_size(int64_t B, int64_t nh, int64_t nkv, int64_t prefix_len,
                                                             int64_t max_len, int with_weights);
 QMOE_API int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void* v_prefix,

@@ -60,7 +60,6 @@ _SIGNATURES = {
                                     ctypes.c_float, P, P, SZ, P]),
     "qmoe_qk_norm_rope_rows": (I32, [P, P, P, P, P, P, P, I64, I64, I64, I64, ctypes.c_float, P, P, P, P, P, I64,
                                      I64, P]),
-    "qmoe_attention_prefix_decode_parts": (I64, [I64, I64, I64, I64, I64]),
     "qmoe_attention_prefix_decode_workspace_size": (SZ, [I64, I64, I64, I64, I64, I32]),
     "qmoe_attention_prefix_decode": (I32, [P, P, P, I64, I64, I64, I64, P, P, P, P, P, I64, I64, I64, I64, I64, I64,
                                            I64, ctypes.c_float, P, I32, P, P, SZ, P]),

@@ -14,7 +14,11 @@
 // log2 units), its sum l of exp2(s - m) and its unnormalised output, which
 // shared_decode_combine_kernel joins:  M = max m,  out = sum_i 2^(m_i - M) o_i
 // / sum_i 2^(m_i - M) l_i.  The joined M and l also turn the scores of the
-// own rows, kept in fp32 by the first kernel, into attention weights.
+// own rows, kept in fp32 by the first kernel, into attention weights.  Own
+// rows are cut by the batch's total: every part of a ragged batch holds about
+// as many rows (cutting each sequence into as many parts took 15 us instead of
+// TODO for 8 sequences of 1,400 to 4,096 rows).  Short calls run as one CTA per
+// (sequence, KV head) over prefix and own rows, without a second kernel.
 #pragma once
 
 #include "attention.cuh"
@@ -40,12 +44,19 @@ struct SharedDecodeArgs {
   const int32_t* kv_len;
   const int32_t* cache_slot;
   const int32_t* kv_start;
-  float* part_o;    // [B*nh][nparts][128]
-  float* part_ml;   // [B*nh][nparts][2]
+  float* pre_o;     // prefix parts [B*nh][psplits][128]
+  float* pre_ml;    // [B*nh][psplits][2]
+  float* own_o;     // own parts [own_cap][nh][128]
+  float* own_ml;    // [own_cap][nh][2]
   float* scores;    // [B*nkv][score_rows][G] log2-scaled scores of the own rows, or null
-  int B, nh, nkv, G, max_seq, max_len, n_slots;
+  float* weights;   // (n_slots, nkv, max_seq) or null
+  __nv_bfloat16* out;
+  int B, nh, nkv, G, max_seq, max_len, n_slots, accumulate;
   int P, prefix_z, psplits, pchunk, row_tiles, n_prefix_units;
-  int osplits, nparts, score_rows;
+  int own_slots;    // parts per KV head that the own rows are cut into (at least one per sequence)
+  int n_own_units, score_rows, n_out_blocks, row_blocks;
+  int direct;       // one unit per (sequence, KV head), nothing to join
+  int overlaps;     // the kernel before it (the tcgen05 prefix part) may still run
   float scale_log2;
 };
 
@@ -62,6 +73,63 @@ __device__ __forceinline__ bool own_range(const int32_t* kv_len, const int32_t* 
   }
   lo = kv_start ? max(0, min(kv_start[b], hi)) : 0;
   return ok;
+}
+
+// How the own rows of a batch are cut, found by every warp for itself: `chunk`
+// rows per part, and for sequence b its first part and their number.
+struct OwnParts {
+  int chunk, first, count;
+};
+__device__ __forceinline__ int own_rows(const SharedDecodeArgs& a, int b) {
+  int slot, lo, hi;
+  own_range(a.kv_len, a.cache_slot, a.kv_start, b, a.max_len, a.n_slots, slot, lo, hi);
+  return hi - lo;
+}
+__device__ __forceinline__ int own_chunk(const SharedDecodeArgs& a, int lane) {
+  long long total = 0;
+  for (int b = lane; b < a.B; b += 32) total += own_rows(a, b);
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, off);
+  const long long c = (total + a.own_slots - 1) / a.own_slots;
+  return max(2 * kSdKeys, int(min(c, (long long)a.max_len) + kSdKeys - 1) / kSdKeys * kSdKeys);
+}
+// The parts of sequence b (part < 0), or the sequence that part `part` belongs
+// to (b out; B when there is no such part).
+__device__ __forceinline__ OwnParts own_parts(const SharedDecodeArgs& a, int& b, int part, int lane) {
+  OwnParts p;
+  p.chunk = own_chunk(a, lane);
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    const int n = b0 + lane < a.B ? (own_rows(a, b0 + lane) + p.chunk - 1) / p.chunk : 0;
+    int incl = n;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int t = __shfl_up_sync(0xFFFFFFFFu, incl, off);
+      if (lane >= off) incl += t;
+    }
+    const bool here = part < 0 ? b0 + lane == b : before + incl > part;
+    const uint32_t hit = __ballot_sync(0xFFFFFFFFu, here);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      if (part >= 0) b = b0 + src;
+      p.first = before + __shfl_sync(0xFFFFFFFFu, incl - n, src);
+      p.count = __shfl_sync(0xFFFFFFFFu, n, src);
+      return p;
+    }
+    before += __shfl_sync(0xFFFFFFFFu, incl, 31);
+  }
+  b = a.B;
+  p.first = p.count = 0;
+  return p;
+}
+
+// Is slot of entry b also the slot of an earlier entry?  (One warp.)
+__device__ __forceinline__ bool slot_seen_before(const int32_t* cache_slot, int b, int lane) {
+  if (!cache_slot) return false;
+  const int mine = cache_slot[b];
+  bool hit = false;
+  for (int i = lane; i < b; i += 32) hit |= cache_slot[i] == mine;
+  return __any_sync(0xFFFFFFFFu, hit);
 }
 
 // One lane of a converged warp, chosen so that the compiler knows it is one: a
@@ -110,7 +178,7 @@ __device__ __forceinline__ void ldsm_x4_trans_at(uint32_t (&r)[4], uint32_t addr
 // 64-key K and V tiles by TMA through three 32 KB stages; four warps take 16
 // keys each (m16n8k16), each with its own running softmax, and are merged in
 // shared memory at the end.  HBM-bound: 2 CTAs per SM hold 192 KB in flight.
-// Ranges begin at their first visible row, so only a part's last tile holds
+// Ranges begin at their first visible row, so only a range's last tile holds
 // foreign rows: their scores are masked and their V fragments zeroed, and a
 // non-finite value there reaches nothing.
 __global__ void __launch_bounds__(kSdThreads)
@@ -118,6 +186,7 @@ __global__ void __launch_bounds__(kSdThreads)
                          const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ CUtensorMap tm_vp,
                          const SharedDecodeArgs a) {
   extern __shared__ uint8_t sd_smem_raw[];
+  __shared__ float2 s_ml[kSdMaxGroup];  // direct: a row's maximum and 1 / l
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sd_smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kSdStages * kSdStageBytes);
   uint64_t* empty = full + kSdStages;
@@ -131,46 +200,57 @@ __global__ void __launch_bounds__(kSdThreads)
     *abort_flag = 0;
     fence_mbarrier_init();
   }
-  const int u = blockIdx.x;
-  const bool prefix = u < a.n_prefix_units;
-  griddep_wait();
+  // The prefix part's kernel reads nothing of this one's and let it start only
+  // after everything before had completed: the two run side by side.
+  if (!a.overlaps) griddep_wait();
   griddep_launch_dependents();
-  // the unit: rows row0 .. row0+n_rows-1 of (sequence, head in group) order, keys [k0, k1)
-  int kvh, part, row0, n_rows, k0, k1, z;
-  int own_b = 0;
-  if (prefix) {
+  // the unit: rows row0 .. row0+n_rows-1 of (sequence, head in group) order over
+  // prefix rows [p0, p1) and own rows [k0, k1)
+  const int u = blockIdx.x;
+  const bool is_prefix = u < a.n_prefix_units;
+  int kvh, part = 0, row0, n_rows, p0 = 0, p1 = 0, k0 = 0, k1 = 0, own_b = 0, slot = 0, lo = 0;
+  bool live = true;
+  if (is_prefix) {
     const int rt = u % a.row_tiles, rest = u / a.row_tiles;
     kvh = rest % a.nkv;
     part = rest / a.nkv;
     row0 = rt * 16;
     n_rows = min(16, a.B * a.G - row0);
-    k0 = part * a.pchunk;
-    k1 = min(a.P, k0 + a.pchunk);
-    z = a.prefix_z + kvh;
+    p0 = part * a.pchunk;
+    p1 = min(a.P, p0 + a.pchunk);
   } else {
     const int v = u - a.n_prefix_units;
-    const int split = v % a.osplits, rest = v / a.osplits;
-    kvh = rest % a.nkv;
-    own_b = rest / a.nkv;
-    part = a.psplits + split;
+    kvh = v % a.nkv;
+    part = v / a.nkv;
+    OwnParts parts = {};
+    if (a.direct)
+      own_b = part;
+    else
+      parts = own_parts(a, own_b, part, lane);
+    live = own_b < a.B;  // there may be fewer parts than units
+    if (live) {
+      int hi;
+      if (!own_range(a.kv_len, a.cache_slot, a.kv_start, own_b, a.max_len, a.n_slots, slot, lo, hi) &&
+          threadIdx.x == 0)
+        record_device_error(kDevErrBadIndex);
+      if (a.direct) {
+        p1 = a.P;
+        k0 = lo;
+        k1 = hi;
+      } else {
+        k0 = lo + (part - parts.first) * parts.chunk;
+        k1 = min(hi, k0 + parts.chunk);
+      }
+    }
     row0 = own_b * a.G;
     n_rows = a.G;
-    int slot, lo, hi;
-    if (!own_range(a.kv_len, a.cache_slot, a.kv_start, own_b, a.max_len, a.n_slots, slot, lo, hi) && threadIdx.x == 0)
-      record_device_error(kDevErrBadIndex);
-    // each sequence splits its own length, so a ragged batch leaves no split idle
-    const int chunk = ((hi - lo + a.osplits - 1) / a.osplits + kSdKeys - 1) / kSdKeys * kSdKeys;
-    k0 = min(hi, lo + split * chunk);
-    k1 = min(hi, k0 + chunk);
-    z = slot * a.nkv + kvh;
   }
-  const int n_tiles = k1 > k0 ? (k1 - k0 + kSdKeys - 1) / kSdKeys : 0;
+  const int n_pre = (p1 - p0 + kSdKeys - 1) / kSdKeys;
+  const int n_tiles = live ? n_pre + (k1 - k0 + kSdKeys - 1) / kSdKeys : 0;
   __syncthreads();
 
   if (warp == 4) {
     if (lane == 0 && n_tiles > 0) {
-      const CUtensorMap* mk = prefix ? &tm_kp : &tm_k;
-      const CUtensorMap* mv = prefix ? &tm_vp : &tm_v;
       int issued = 0;
       for (int j = 0; j < n_tiles; ++j, ++issued) {
         const int st = j % kSdStages;
@@ -178,7 +258,11 @@ __global__ void __launch_bounds__(kSdThreads)
             !mbar_wait_bounded(&empty[st], (j / kSdStages - 1) & 1, abort_flag, kDevErrWaitTimeoutProducer))
           break;
         uint8_t* kt = smem + st * kSdStageBytes;
-        const int y = k0 + j * kSdKeys;
+        const bool pre = j < n_pre;
+        const CUtensorMap* mk = pre ? &tm_kp : &tm_k;
+        const CUtensorMap* mv = pre ? &tm_vp : &tm_v;
+        const int y = pre ? p0 + j * kSdKeys : k0 + (j - n_pre) * kSdKeys;
+        const int z = pre ? a.prefix_z + kvh : slot * a.nkv + kvh;
         mbar_arrive_expect_tx(&full[st], kSdStageBytes);
         tma_load_3d(kt, mk, 0, y, z, &full[st]);
         tma_load_3d(kt + kSdHalfBytes, mk, 64, y, z, &full[st]);
@@ -194,7 +278,7 @@ __global__ void __launch_bounds__(kSdThreads)
   float o[16][4];
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   bool ok = true;
-  if (warp < 4) {
+  if (warp < 4 && n_tiles > 0) {
     // query fragments straight from global memory; rows past n_rows are zero
     uint32_t qa[8][4];
 #pragma unroll
@@ -212,7 +296,7 @@ __global__ void __launch_bounds__(kSdThreads)
     for (int dn = 0; dn < 16; ++dn)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[dn][i] = 0.f;
-    float* sc_out = (!prefix && a.scores) ? a.scores + size_t(own_b * a.nkv + kvh) * a.score_rows * a.G : nullptr;
+    float* sc_out = a.scores ? a.scores + size_t(own_b * a.nkv + kvh) * a.score_rows * a.G : nullptr;
     const int mi = lane >> 3, r8 = lane & 7;
     for (int j = 0; j < n_tiles; ++j) {
       const int st = j % kSdStages;
@@ -220,8 +304,10 @@ __global__ void __launch_bounds__(kSdThreads)
         ok = false;
         break;
       }
-      const int key0 = k0 + j * kSdKeys + warp * 16;
-      if (key0 < k1) {
+      const bool pre = j < n_pre;
+      const int end = pre ? p1 : k1;
+      const int key0 = (pre ? p0 + j * kSdKeys : k0 + (j - n_pre) * kSdKeys) + warp * 16;
+      if (key0 < end) {
         const uint32_t kt = smem_u32(smem + st * kSdStageBytes), vt = kt + kSdTileBytes;
         float s[2][4];
 #pragma unroll
@@ -236,21 +322,21 @@ __global__ void __launch_bounds__(kSdThreads)
             mma_bf16_16816(s[nt], qa[kk + 1], b[2], b[3]);
           }
         }
-        const bool tail = key0 + 16 > k1;
+        const bool tail = key0 + 16 > end;
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             s[nt][i] *= a.scale_log2;
-            if (tail && key0 + nt * 8 + 2 * tq + (i & 1) >= k1) s[nt][i] = -INFINITY;
+            if (tail && key0 + nt * 8 + 2 * tq + (i & 1) >= end) s[nt][i] = -INFINITY;
           }
-        if (sc_out) {
+        if (sc_out && !pre) {
 #pragma unroll
           for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int key = key0 + nt * 8 + 2 * tq + (i & 1), row = g + 8 * (i >> 1);
-              if (key < k1 && row < n_rows) sc_out[size_t(key) * a.G + row] = s[nt][i];
+              if (key < end && row < n_rows) sc_out[size_t(key) * a.G + row] = s[nt][i];
             }
         }
         float alpha[2];
@@ -281,7 +367,7 @@ __global__ void __launch_bounds__(kSdThreads)
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[dn][i] *= alpha[i >> 1];
         }
-        // P in bf16 (in [0, 1], relative rounding 2^-9): the tensor core's operand type
+        // P in bf16 (in [0, 1], relative rounding 2^-8): the tensor core's operand type
         uint32_t pa[4];
         pa[0] = pack_bf16x2(s[0][0], s[0][1]);
         pa[1] = pack_bf16x2(s[0][2], s[0][3]);
@@ -290,8 +376,8 @@ __global__ void __launch_bounds__(kSdThreads)
         uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;  // V rows of this lane's keys
         if (tail) {
           const int ka = key0 + 2 * tq;
-          keep0 = (ka < k1 ? 0xFFFFu : 0u) | (ka + 1 < k1 ? 0xFFFF0000u : 0u);
-          keep1 = (ka + 8 < k1 ? 0xFFFFu : 0u) | (ka + 9 < k1 ? 0xFFFF0000u : 0u);
+          keep0 = (ka < end ? 0xFFFFu : 0u) | (ka + 1 < end ? 0xFFFF0000u : 0u);
+          keep1 = (ka + 8 < end ? 0xFFFFu : 0u) | (ka + 9 < end ? 0xFFFF0000u : 0u);
         }
 #pragma unroll
         for (int dn = 0; dn < 16; dn += 2) {
@@ -312,99 +398,132 @@ __global__ void __launch_bounds__(kSdThreads)
   }
   // every load has landed and been read: the stages hold the warps' results now
   const bool all_ok = __syncthreads_and(ok) != 0;
-  if (!all_ok) return;
-  float* red = reinterpret_cast<float*>(smem);
-  if (warp < 4 && n_tiles > 0) {
+  if (all_ok && live) {
+    float* red = reinterpret_cast<float*>(smem);
+    if (warp < 4 && n_tiles > 0) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float* wr = red + (warp * 16 + g + 8 * h) * kSdRedStride;
+      for (int h = 0; h < 2; ++h) {
+        float* wr = red + (warp * 16 + g + 8 * h) * kSdRedStride;
 #pragma unroll
-      for (int dn = 0; dn < 16; ++dn)
-        *reinterpret_cast<float2*>(wr + dn * 8 + 2 * tq) = make_float2(o[dn][2 * h], o[dn][2 * h + 1]);
-      if (tq == 0) *reinterpret_cast<float2*>(wr + kAttnD) = make_float2(m[h], l[h]);
-    }
-  }
-  __syncthreads();
-  if (warp >= 4) return;
-  // eight threads per row, 16 dims each
-  const int i = threadIdx.x >> 3, d0 = (threadIdx.x & 7) * 16;
-  if (i >= n_rows) return;
-  const int r = row0 + i;
-  const size_t pidx = (size_t(r / a.G) * a.nh + kvh * a.G + r % a.G) * a.nparts + part;
-  float M = -INFINITY, L = 0.f;
-  if (n_tiles > 0) {
-#pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, red[(w * 16 + i) * kSdRedStride + kAttnD]);
-    const float base = M == -INFINITY ? 0.f : M;
-    float acc[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float* rw = red + (w * 16 + i) * kSdRedStride;
-      const float sc = exp2f(rw[kAttnD] - base);
-      L += rw[kAttnD + 1] * sc;
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(rw + d0 + e);
-        acc[e] += v.x * sc;
-        acc[e + 1] += v.y * sc;
-        acc[e + 2] += v.z * sc;
-        acc[e + 3] += v.w * sc;
+        for (int dn = 0; dn < 16; ++dn)
+          *reinterpret_cast<float2*>(wr + dn * 8 + 2 * tq) = make_float2(o[dn][2 * h], o[dn][2 * h + 1]);
+        if (tq == 0) *reinterpret_cast<float2*>(wr + kAttnD) = make_float2(m[h], l[h]);
       }
     }
-    float4* po = reinterpret_cast<float4*>(a.part_o + pidx * kAttnD + d0);
+    __syncthreads();
+    // eight threads per row, 16 dims each
+    const int i = threadIdx.x >> 3, d0 = (threadIdx.x & 7) * 16;
+    if (warp < 4 && i < n_rows) {
+      const int r = row0 + i;
+      const int bh = r / a.G * a.nh + kvh * a.G + r % a.G;
+      float M = -INFINITY, L = 0.f;
+      float acc[16];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) po[e] = make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
+      for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+      if (n_tiles > 0) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, red[(w * 16 + i) * kSdRedStride + kAttnD]);
+        const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float* rw = red + (w * 16 + i) * kSdRedStride;
+          const float sc = exp2f(rw[kAttnD] - base);
+          L += rw[kAttnD + 1] * sc;
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(rw + d0 + e);
+            acc[e] += v.x * sc;
+            acc[e + 1] += v.y * sc;
+            acc[e + 2] += v.z * sc;
+            acc[e + 3] += v.w * sc;
+          }
+        }
+      }
+      if (a.direct) {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        uint4* po = reinterpret_cast<uint4*>(a.out + size_t(bh) * kAttnD + d0);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          po[e] = make_uint4(pack_bf16x2(acc[8 * e] * inv, acc[8 * e + 1] * inv),
+                             pack_bf16x2(acc[8 * e + 2] * inv, acc[8 * e + 3] * inv),
+                             pack_bf16x2(acc[8 * e + 4] * inv, acc[8 * e + 5] * inv),
+                             pack_bf16x2(acc[8 * e + 6] * inv, acc[8 * e + 7] * inv));
+        if (d0 == 0) s_ml[i] = make_float2(M == -INFINITY ? 0.f : M, inv);
+      } else {
+        const size_t pidx = is_prefix ? size_t(bh) * a.psplits + part : size_t(part) * a.nh + kvh * a.G + i;
+        float4* po = reinterpret_cast<float4*>((is_prefix ? a.pre_o : a.own_o) + pidx * kAttnD + d0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) po[e] = make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
+        if (d0 == 0) *reinterpret_cast<float2*>((is_prefix ? a.pre_ml : a.own_ml) + pidx * 2) = make_float2(M, L);
+      }
+    }
+    if (a.direct && a.weights) {
+      const bool dup = slot_seen_before(a.cache_slot, own_b, lane);  // two entries of one slot would race
+      __syncthreads();  // the scores and s_ml are there
+      if (dup) {
+        if (threadIdx.x == 0) record_device_error(kDevErrBadIndex);
+      } else {
+        float* w = a.weights + (size_t(slot) * a.nkv + kvh) * a.max_seq;
+        const float* sc = a.scores + size_t(own_b * a.nkv + kvh) * a.score_rows * a.G;
+        for (int row = (a.accumulate ? lo : 0) + threadIdx.x; row < k1; row += kSdThreads) {
+          float x = 0.f;
+          if (row >= lo)
+            for (int h = 0; h < a.G; ++h) x += exp2f(sc[size_t(row) * a.G + h] - s_ml[h].x) * s_ml[h].y;
+          w[row] = a.accumulate ? w[row] + x : x;
+        }
+      }
+    }
   }
-  // an empty part has l = 0; its output is not written and never read
-  if (d0 == 0) *reinterpret_cast<float2*>(a.part_ml + pidx * 2) = make_float2(M, L);
+  // the grid completes after the kernel before it, for the one that joins both
+  if (a.overlaps && blockIdx.x == gridDim.x - 1) griddep_wait();
 }
 
-struct SharedCombineArgs {
-  const float* part_o;
-  const float* part_ml;
-  const float* scores;
-  const int32_t* kv_len;
-  const int32_t* cache_slot;
-  const int32_t* kv_start;
-  float* weights;   // (n_slots, nkv, max_seq) or null
-  __nv_bfloat16* out;
-  int B, nh, nkv, G, nparts, n_out_blocks, row_blocks, score_rows, max_len, max_seq, n_slots, accumulate;
+// A row's parts: the prefix's, then its own.
+struct RowParts {
+  const float* pre_ml;
+  const float* pre_o;
+  const float* own_ml;  // of the sequence's first part
+  const float* own_o;
+  int n_pre, n, nh;
+  __device__ __forceinline__ float2 ml(int i) const {
+    return *reinterpret_cast<const float2*>(i < n_pre ? pre_ml + i * 2 : own_ml + size_t(i - n_pre) * nh * 2);
+  }
+  __device__ __forceinline__ float4 o(int i, int lane) const {
+    return *reinterpret_cast<const float4*>((i < n_pre ? pre_o + size_t(i) * kAttnD
+                                                       : own_o + size_t(i - n_pre) * nh * kAttnD) +
+                                            lane * 4);
+  }
 };
+__device__ __forceinline__ RowParts row_parts(const SharedDecodeArgs& a, const OwnParts& own, int b, int h) {
+  const size_t bh = size_t(b) * a.nh + h, first = size_t(own.first) * a.nh + h;
+  return {a.pre_ml + bh * a.psplits * 2, a.pre_o + bh * a.psplits * kAttnD, a.own_ml + first * 2,
+          a.own_o + first * kAttnD,      a.psplits, a.psplits + own.count,  a.nh};
+}
 
 // M and 1/l of one row from its parts, in every lane of the warp.
-__device__ __forceinline__ void join_ml(const float* part_ml, size_t base, int nparts, int lane, float& M,
-                                        float& inv_l) {
-  float mm = -INFINITY;
-  for (int s = lane; s < nparts; s += 32) mm = fmaxf(mm, part_ml[(base + s) * 2]);
+__device__ __forceinline__ void join_ml(const RowParts& p, int lane, float& M, float& inv_l) {
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (lane < p.n) ml = p.ml(lane);
+  float mm = ml.x;
+  for (int s = lane + 32; s < p.n; s += 32) mm = fmaxf(mm, p.ml(s).x);
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, off));
   M = mm == -INFINITY ? 0.f : mm;
-  float L = 0.f;
-  for (int s = lane; s < nparts; s += 32) {
-    const float2 ml = *reinterpret_cast<const float2*>(part_ml + (base + s) * 2);
-    if (ml.y != 0.f) L += ml.y * exp2f(ml.x - M);
+  float L = ml.y == 0.f ? 0.f : ml.y * exp2f(ml.x - M);
+  for (int s = lane + 32; s < p.n; s += 32) {
+    const float2 v = p.ml(s);
+    if (v.y != 0.f) L += v.y * exp2f(v.x - M);
   }
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) L += __shfl_xor_sync(0xFFFFFFFFu, L, off);
   inv_l = L == 0.f ? 0.f : 1.f / L;
 }
 
-// Is slot of entry b also the slot of an earlier entry?  (One warp.)
-__device__ __forceinline__ bool slot_seen_before(const int32_t* cache_slot, int b, int lane) {
-  if (!cache_slot) return false;
-  const int mine = cache_slot[b];
-  bool hit = false;
-  for (int i = lane; i < b; i += 32) hit |= cache_slot[i] == mine;
-  return __any_sync(0xFFFFFFFFu, hit);
-}
-
 // Blocks [0, n_out_blocks): one warp per (sequence, head) joins the parts of
 // its output row in part order (run-to-run identical).  The blocks after
 // them: 256 own rows of one (sequence, KV head) each, one thread per row,
 // weights (+)= sum over the group's heads of exp2(s - M) / l.
-__global__ void __launch_bounds__(256) shared_decode_combine_kernel(const SharedCombineArgs a) {
+__global__ void __launch_bounds__(256) shared_decode_combine_kernel(const SharedDecodeArgs a) {
   __shared__ float sM[kSdMaxGroup], sInv[kSdMaxGroup];
   __shared__ int s_dup;
   griddep_wait();
@@ -413,26 +532,25 @@ __global__ void __launch_bounds__(256) shared_decode_combine_kernel(const Shared
   if (int(blockIdx.x) < a.n_out_blocks) {
     const int gw = blockIdx.x * 8 + warp;
     if (gw >= a.B * a.nh) return;
-    const size_t base = size_t(gw) * a.nparts;
+    int b = gw / a.nh;
+    const OwnParts own = own_parts(a, b, -1, lane);
+    const RowParts p = row_parts(a, own, b, gw % a.nh);
     float M, inv;
-    join_ml(a.part_ml, base, a.nparts, lane, M, inv);
+    join_ml(p, lane, M, inv);
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < a.nparts; s0 += 8) {
+    for (int s0 = 0; s0 < p.n; s0 += 8) {
       float4 v[8];
       float sc[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         sc[j] = 0.f;
-        if (s0 + j < a.nparts) {
-          const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (base + s0 + j) * 2);
-          if (ml.y != 0.f) {
+        v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (s0 + j < p.n) {
+          const float2 ml = p.ml(s0 + j);
+          if (ml.y != 0.f) {  // an empty part has no output
             sc[j] = exp2f(ml.x - M);
-            v[j] = *reinterpret_cast<const float4*>(a.part_o + (base + s0 + j) * kAttnD + lane * 4);
-          } else {
-            v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            v[j] = p.o(s0 + j, lane);
           }
-        } else {
-          v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
 #pragma unroll
@@ -451,14 +569,16 @@ __global__ void __launch_bounds__(256) shared_decode_combine_kernel(const Shared
   }
   const int v = blockIdx.x - a.n_out_blocks;
   const int rb = v % a.row_blocks, rest = v / a.row_blocks;
-  const int kvh = rest % a.nkv, b = rest / a.nkv;
+  const int kvh = rest % a.nkv;
+  int b = rest / a.nkv;
   int slot, lo, hi;
   if (!own_range(a.kv_len, a.cache_slot, a.kv_start, b, a.max_len, a.n_slots, slot, lo, hi)) return;  // recorded before
   const int first = rb * kSdCombineRows;
   if (first >= hi) return;
+  const OwnParts own = own_parts(a, b, -1, lane);
   for (int h = warp; h < a.G; h += 8) {
     float M, inv;
-    join_ml(a.part_ml, (size_t(b) * a.nh + kvh * a.G + h) * a.nparts, a.nparts, lane, M, inv);
+    join_ml(row_parts(a, own, b, kvh * a.G + h), lane, M, inv);
     if (lane == 0) {
       sM[h] = M;
       sInv[h] = inv;

@@ -950,8 +950,13 @@ bool flash_prefix_split(int64_t row_tiles, int64_t columns, double key_tiles, in
 struct SharedDecodePlan {
   bool tc, split;      // the prefix part runs on the tcgen05 kernel, and splits its key tiles
   int64_t row_tiles;   // 16-row tiles, or the tcgen05 kernel's row blocks, of one KV head's rows
-  int64_t psplits, pchunk, osplits;
+  int64_t psplits, pchunk;
+  int64_t own_slots, own_cap;  // parts per KV head aimed at, and at most
+  bool direct;         // one CTA per (sequence, KV head) does it all
 };
+
+// Rows (prefix and own) up to which a sequence's keys are not cut.
+constexpr int64_t kDirectRows = 512;
 
 // Rows (sequences x heads of a group) above which the prefix part runs on the
 // tcgen05 kernel.
@@ -961,6 +966,8 @@ SharedDecodePlan shared_decode_plan(int64_t B, int64_t G, int64_t nkv, int64_t P
   SharedDecodePlan p{};
   const int64_t sms = std::max(1, num_sms(0));
   const int64_t rows = B * G;
+  p.direct = P + max_len <= kDirectRows;
+  if (p.direct) return p;
   p.tc = P > 0 && rows > kPrefixMmaRows;
   if (p.tc) {
     // one CTA per SM; the split form where it leaves a CTA fewer steps
@@ -988,8 +995,11 @@ SharedDecodePlan shared_decode_plan(int64_t B, int64_t G, int64_t nkv, int64_t P
     p.pchunk = ((P + want - 1) / want + qmoe::kSdKeys - 1) / qmoe::kSdKeys * qmoe::kSdKeys;
     p.psplits = (P + p.pchunk - 1) / p.pchunk;
   }
-  if (max_len > 0)
-    p.osplits = std::max<int64_t>(1, std::min((2 * sms + B * nkv - 1) / (B * nkv), (max_len + 127) / 128));
+  if (max_len > 0) {
+    // two CTAs per SM; every sequence has a part of its own, none shorter than 128 rows but its last
+    p.own_slots = std::max<int64_t>(1, 2 * sms / nkv);
+    p.own_cap = std::min(p.own_slots + B, B * ((max_len + 127) / 128));
+  }
   return p;
 }
 
@@ -1572,20 +1582,12 @@ int qmoe_attention_decode(const void* q, const void* k_cache, const void* v_cach
                        static_cast<__nv_bfloat16*>(out));
 }
 
-int64_t qmoe_attention_prefix_decode_parts(int64_t B, int64_t nh, int64_t nkv, int64_t prefix_len, int64_t max_len) {
-  if (B <= 0 || nkv <= 0 || nh <= 0 || nh % nkv != 0) return 0;
-  const SharedDecodePlan p = shared_decode_plan(B, nh / nkv, nkv, std::max<int64_t>(prefix_len, 0),
-                                                std::max<int64_t>(max_len, 0));
-  return p.psplits + p.osplits;
-}
-
 size_t qmoe_attention_prefix_decode_workspace_size(int64_t B, int64_t nh, int64_t nkv, int64_t prefix_len,
                                                    int64_t max_len, int with_weights) {
-  const size_t parts = size_t(qmoe_attention_prefix_decode_parts(B, nh, nkv, prefix_len, max_len));
-  if (B <= 0 || nh <= 0) return 0;
-  return size_t(B * nh) * (parts * (qmoe::kAttnD + 2) + (with_weights ? size_t(std::max<int64_t>(max_len, 0)) : 0)) *
-             sizeof(float) +
-         256;
+  if (B <= 0 || nkv <= 0 || nh <= 0 || nh % nkv != 0 || prefix_len < 0 || max_len < 0) return 0;
+  const SharedDecodePlan p = shared_decode_plan(B, nh / nkv, nkv, prefix_len, max_len);
+  const size_t rows = size_t(B * nh * p.psplits + p.own_cap * nh);
+  return (rows * (qmoe::kAttnD + 2) + (with_weights ? size_t(B * nh) * size_t(max_len) : 0)) * sizeof(float) + 256;
 }
 
 int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void* v_prefix, int64_t n_prefix_slots,
@@ -1612,11 +1614,13 @@ int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void
   if (B == 0) return QMOE_OK;
   const int64_t G = nh / nkv;
   const SharedDecodePlan p = shared_decode_plan(B, G, nkv, prefix_len, max_len);
-  const int64_t nparts = p.psplits + p.osplits;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  float* part_o = static_cast<float*>(workspace);
-  float* part_ml = part_o + size_t(B * nh * nparts) * qmoe::kAttnD;
-  float* scores = part_ml + size_t(B * nh * nparts) * 2;
+  qmoe::SharedDecodeArgs a{};
+  a.pre_o = static_cast<float*>(workspace);
+  a.own_o = a.pre_o + size_t(B * nh * p.psplits) * qmoe::kAttnD;
+  a.pre_ml = a.own_o + size_t(p.own_cap * nh) * qmoe::kAttnD;
+  a.own_ml = a.pre_ml + size_t(B * nh * p.psplits) * 2;
+  a.scores = weights ? a.own_ml + size_t(p.own_cap * nh) * 2 : nullptr;
   CUtensorMap tk, tv, tkp, tvp;
   QMOE_CHECK(make_tmap_rows(&tk, k_cache, max_seq, max_seq, n_slots * nkv, qmoe::kSdKeys));
   QMOE_CHECK(make_tmap_rows(&tv, v_cache, max_seq, max_seq, n_slots * nkv, qmoe::kSdKeys));
@@ -1629,8 +1633,8 @@ int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void
     QMOE_CHECK(make_tmap_rows(&tk128, k_prefix, prefix_len, prefix_max, n_prefix_slots * nkv, qmoe::kFaRows));
     QMOE_CHECK(make_tmap_rows(&tv128, v_prefix, prefix_len, prefix_max, n_prefix_slots * nkv, qmoe::kFaRows));
     qmoe::FlashPrefixArgs fa{};
-    fa.part_o = part_o;
-    fa.part_ml = part_ml;
+    fa.part_o = a.pre_o;
+    fa.part_ml = a.pre_ml;
     fa.nh = int(nh);
     fa.nkv = int(nkv);
     fa.B = int(B);
@@ -1638,7 +1642,7 @@ int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void
     fa.P = int(prefix_len);
     fa.prefix_z = int(prefix_slot * nkv);
     fa.G = int(G);
-    fa.nparts = int(nparts);
+    fa.nparts = int(p.psplits);
     fa.tiles_per_part = int(p.pchunk / qmoe::kFaRows);
     fa.scale_log2 = scale * 1.4426950408889634f;
     QMOE_CHECK(launch_flash_prefix(true, p.split, p.row_tiles * nkv * p.psplits, tq, tk128, tv128, tk128, tv128, fa, s));
@@ -1646,14 +1650,12 @@ int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void
     QMOE_CHECK(make_tmap_rows(&tkp, k_prefix, prefix_len, prefix_max, n_prefix_slots * nkv, qmoe::kSdKeys));
     QMOE_CHECK(make_tmap_rows(&tvp, v_prefix, prefix_len, prefix_max, n_prefix_slots * nkv, qmoe::kSdKeys));
   }
-  qmoe::SharedDecodeArgs a{};
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.kv_len = kv_len;
   a.cache_slot = cache_slot;
   a.kv_start = kv_start;
-  a.part_o = part_o;
-  a.part_ml = part_ml;
-  a.scores = weights ? scores : nullptr;
+  a.weights = weights;
+  a.out = static_cast<__nv_bfloat16*>(out);
   a.B = int(B);
   a.nh = int(nh);
   a.nkv = int(nkv);
@@ -1661,46 +1663,31 @@ int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void
   a.max_seq = int(max_seq);
   a.max_len = int(max_len);
   a.n_slots = int(n_slots);
+  a.accumulate = accumulate ? 1 : 0;
   a.P = int(prefix_len);
   a.prefix_z = int(prefix_slot * nkv);
   a.psplits = int(p.psplits);
   a.pchunk = int(p.pchunk);
   a.row_tiles = int(p.row_tiles);
   a.n_prefix_units = p.tc ? 0 : int(p.row_tiles * nkv * p.psplits);
-  a.osplits = int(p.osplits);
-  a.nparts = int(nparts);
+  a.own_slots = int(p.own_slots);
+  a.n_own_units = int((p.direct ? B : p.own_cap) * nkv);
   a.score_rows = int(max_len);
+  a.n_out_blocks = int((B * nh + 7) / 8);
+  a.row_blocks = int((max_len + qmoe::kSdCombineRows - 1) / qmoe::kSdCombineRows);
+  a.direct = p.direct ? 1 : 0;
+  a.overlaps = p.tc ? 1 : 0;
   a.scale_log2 = scale * 1.4426950408889634f;
-  const int64_t units = a.n_prefix_units + B * nkv * p.osplits;
+  const int64_t units = int64_t(a.n_prefix_units) + a.n_own_units;
   if (units > 0) {
     QMOE_CHECK(set_smem(qmoe::shared_decode_kernel, qmoe::kSdSmemBytes));
     QMOE_CHECK(launch_kernel(qmoe::shared_decode_kernel, dim3(unsigned(units)), dim3(qmoe::kSdThreads),
                              size_t(qmoe::kSdSmemBytes), s, true, "shared_decode_kernel", tk, tv, tkp, tvp, a));
   }
-  qmoe::SharedCombineArgs c{};
-  c.part_o = part_o;
-  c.part_ml = part_ml;
-  c.scores = scores;
-  c.kv_len = kv_len;
-  c.cache_slot = cache_slot;
-  c.kv_start = kv_start;
-  c.weights = weights;
-  c.out = static_cast<__nv_bfloat16*>(out);
-  c.B = int(B);
-  c.nh = int(nh);
-  c.nkv = int(nkv);
-  c.G = int(G);
-  c.nparts = int(nparts);
-  c.n_out_blocks = int((B * nh + 7) / 8);
-  c.row_blocks = int((max_len + qmoe::kSdCombineRows - 1) / qmoe::kSdCombineRows);
-  c.score_rows = int(max_len);
-  c.max_len = int(max_len);
-  c.max_seq = int(max_seq);
-  c.n_slots = int(n_slots);
-  c.accumulate = accumulate ? 1 : 0;
-  const int64_t blocks = c.n_out_blocks + (weights ? B * nkv * c.row_blocks : 0);
+  if (p.direct) return QMOE_OK;
+  const int64_t blocks = a.n_out_blocks + (weights ? B * nkv * a.row_blocks : 0);
   return launch_kernel(qmoe::shared_decode_combine_kernel, dim3(unsigned(blocks)), dim3(256), 0, s, true,
-                       "shared_decode_combine_kernel", c);
+                       "shared_decode_combine_kernel", a);
 }
 
 int qmoe_attention_prefix_prefill(const void* q, const void* k_prefix, const void* v_prefix, int64_t n_prefix_slots,

@@ -97,7 +97,7 @@ def _decode(lib, p, **kw):
     (dict(P=-1), -1), (dict(P=65), -1), (dict(slot=1), -1), (dict(slot=-1), -1),
     (dict(max_len=65), -1), (dict(max_len=-1), -1), (dict(B=3), -1), (dict(B=-1), -1),
     (dict(scale=0.0), -1), (dict(scale=-1.0), -1), (dict(scale=float("inf")), -1), (dict(scale=float("nan")), -1),
-    (dict(bytes=1000), -4), (dict(n_slots=0), -1),
+    (dict(bytes=255), -4), (dict(n_slots=0), -1),
 ])
 def test_decode_refusals(lib, p, kw, status):
     assert _decode(lib, p, **kw) == status

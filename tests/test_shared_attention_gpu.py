@@ -89,6 +89,10 @@ DECODE = [
     (70, 2, 2, 127, [3] * 70, None, None, 0),
     (2, 32, 4, 5000, [4096, 700], None, None, 0),              # many parts
     (130, 8, 8, 700, [1] * 130, None, None, 0),                # one head per KV head
+    (4, 32, 4, 0, [700, 0, 1300, 129], [0, 0, 700, 128], [3, 1, 0, 2], 0),
+    (2, 48, 3, 450, [63, 5], [0, 5], None, 0),
+    (40, 16, 4, 0, [20 * i for i in range(40)], None, None, 0),
+    (1, 16, 16, 0, [9000], [1], None, 0),
 ]
 
 
