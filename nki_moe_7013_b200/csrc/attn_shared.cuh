@@ -81,26 +81,25 @@ struct OwnParts {
   int chunk, first, count;
 };
 __device__ __forceinline__ int own_rows(const SharedDecodeArgs& a, int b) {
+  if (b >= a.B) return 0;
   int slot, lo, hi;
   own_range(a.kv_len, a.cache_slot, a.kv_start, b, a.max_len, a.n_slots, slot, lo, hi);
   return hi - lo;
 }
-__device__ __forceinline__ int own_chunk(const SharedDecodeArgs& a, int lane) {
-  long long total = 0;
-  for (int b = lane; b < a.B; b += 32) total += own_rows(a, b);
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, off);
-  const long long c = (total + a.own_slots - 1) / a.own_slots;
-  return max(2 * kSdKeys, int(min(c, (long long)a.max_len) + kSdKeys - 1) / kSdKeys * kSdKeys);
-}
 // The parts of sequence b (part < 0), or the sequence that part `part` belongs
 // to (b out; B when there is no such part).
 __device__ __forceinline__ OwnParts own_parts(const SharedDecodeArgs& a, int& b, int part, int lane) {
+  const int first_rows = own_rows(a, lane);  // of the first 32 sequences: read once
+  long long total = first_rows;
+  for (int i = lane + 32; i < a.B; i += 32) total += own_rows(a, i);
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, off);
   OwnParts p;
-  p.chunk = own_chunk(a, lane);
+  const long long even = (total + a.own_slots - 1) / a.own_slots;
+  p.chunk = max(2 * kSdKeys, (int(min(even, (long long)a.max_len)) + kSdKeys - 1) / kSdKeys * kSdKeys);
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 32) {
-    const int n = b0 + lane < a.B ? (own_rows(a, b0 + lane) + p.chunk - 1) / p.chunk : 0;
+    const int n = ((b0 == 0 ? first_rows : own_rows(a, b0 + lane)) + p.chunk - 1) / p.chunk;
     int incl = n;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -199,6 +198,12 @@ __global__ void __launch_bounds__(kSdThreads)
     }
     *abort_flag = 0;
     fence_mbarrier_init();
+  }
+  if (threadIdx.x == 128) {
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+    prefetch_tmap(&tm_kp);
+    prefetch_tmap(&tm_vp);
   }
   // The prefix part's kernel reads nothing of this one's and let it start only
   // after everything before had completed: the two run side by side.
@@ -309,25 +314,27 @@ __global__ void __launch_bounds__(kSdThreads)
       const int key0 = (pre ? p0 + j * kSdKeys : k0 + (j - n_pre) * kSdKeys) + warp * 16;
       if (key0 < end) {
         const uint32_t kt = smem_u32(smem + st * kSdStageBytes), vt = kt + kSdTileBytes;
-        float s[2][4];
+        // four independent chains of MMAs (a chain of eight waits on itself)
+        float s[2][4], s1[2][4];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
+        for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
+          for (int i = 0; i < 4; ++i) s[nt][i] = s1[nt][i] = 0.f;
 #pragma unroll
-          for (int kk = 0; kk < 8; kk += 2) {
+        for (int kk = 0; kk < 8; kk += 2)
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) {
             uint32_t b[4];
             ldsm_x4_at(b, sw128_addr(kt, warp * 16 + nt * 8 + r8, kk * 2 + mi));
             mma_bf16_16816(s[nt], qa[kk], b[0], b[1]);
-            mma_bf16_16816(s[nt], qa[kk + 1], b[2], b[3]);
+            mma_bf16_16816(s1[nt], qa[kk + 1], b[2], b[3]);
           }
-        }
         const bool tail = key0 + 16 > end;
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            s[nt][i] *= a.scale_log2;
+            s[nt][i] = (s[nt][i] + s1[nt][i]) * a.scale_log2;
             if (tail && key0 + nt * 8 + 2 * tq + (i & 1) >= end) s[nt][i] = -INFINITY;
           }
         if (sc_out && !pre) {
@@ -339,35 +346,43 @@ __global__ void __launch_bounds__(kSdThreads)
               if (key < end && row < n_rows) sc_out[size_t(key) * a.G + row] = s[nt][i];
             }
         }
-        float alpha[2];
-        bool grew = false;
+        // The running maximum moves only when a score exceeds it by more than
+        // 2^8: the exponentials stay below 2^8, and most tiles need no
+        // exchange between lanes and no rescaling.  Rows 8..15 are idle with
+        // up to 8 rows.
+        float mx[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float mx = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
-          const float m_new = fmaxf(m[h], mx);
-          const float base = m_new == -INFINITY ? 0.f : m_new;
-          alpha[h] = exp2f(m[h] - base);  // m[h] == -inf -> 0
-          grew |= m_new != m[h];
-          m[h] = m_new;
-          float sum = 0.f;
+        for (int h = 0; h < 2; ++h) mx[h] = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+        if (__any_sync(0xFFFFFFFFu, mx[0] > m[0] + kFaRescaleLog2 || (n_rows > 8 && mx[1] > m[1] + kFaRescaleLog2))) {
+          float alpha[2];
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              s[nt][2 * h + e] = exp2f(s[nt][2 * h + e] - base);
-              sum += s[nt][2 * h + e];
-            }
-          l[h] = l[h] * alpha[h] + sum;
-        }
-        if (__any_sync(0xFFFFFFFFu, grew)) {
+          for (int h = 0; h < 2; ++h) {
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xFFFFFFFFu, mx[h], 1));
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xFFFFFFFFu, mx[h], 2));
+            const float m_new = fmaxf(m[h], mx[h]);
+            alpha[h] = fa_exp2(m[h] - (m_new == -INFINITY ? 0.f : m_new));  // m[h] == -inf -> 0
+            m[h] = m_new;
+            l[h] *= alpha[h];
+          }
 #pragma unroll
           for (int dn = 0; dn < 16; ++dn)
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[dn][i] *= alpha[i >> 1];
         }
-        // P in bf16 (in [0, 1], relative rounding 2^-8): the tensor core's operand type
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h == 1 && n_rows <= 8) {
+            s[0][2] = s[0][3] = s[1][2] = s[1][3] = 0.f;
+            continue;
+          }
+          const float base = m[h] == -INFINITY ? 0.f : m[h];
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) s[nt][2 * h + e] = fa_exp2(s[nt][2 * h + e] - base);
+          l[h] += (s[0][2 * h] + s[0][2 * h + 1]) + (s[1][2 * h] + s[1][2 * h + 1]);
+        }
+        // P in bf16 (in [0, 2^8], relative rounding 2^-8): the tensor core's operand type
         uint32_t pa[4];
         pa[0] = pack_bf16x2(s[0][0], s[0][1]);
         pa[1] = pack_bf16x2(s[0][2], s[0][3]);

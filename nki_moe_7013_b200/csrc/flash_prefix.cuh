@@ -95,6 +95,13 @@ __global__ void __launch_bounds__(kFaThreads, 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tm_q);
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+    prefetch_tmap(&tm_kp);
+    prefetch_tmap(&tm_vp);
+  }
   griddep_wait();
   if (kPartial) griddep_launch_dependents();
 
