@@ -20,14 +20,14 @@
 //
 // Four K tiles per query tile because the query tiles come from L2: with one,
 // a 4,096-token prompt read 550 MB through it, and ran at that rate (93 us
-// without any arithmetic).  Then the exponentials bound it (128 x 128 per tile
-// at 16 a cycle and SM: 1,024 cycles, against 512 of the products), so
-// kAwPoly of 8 columns take theirs on the FMA pipe.
+// without any arithmetic).  Then the exponentials bound it: 128 x 128 per tile
+// at 16 a cycle and SM are 1,024 cycles, against 512 of the products.  (A
+// quarter or a half of them as a degree-5 polynomial on the FMA pipe changed
+// nothing or cost 5 %: ten multiply-adds take as long as they save.)
 #pragma once
 
 #include "attn_shared.cuh"
 #include "common.cuh"
-#include "fast_exp2.cuh"
 #include "flash_prefill.cuh"
 
 namespace qmoe {
@@ -40,10 +40,6 @@ constexpr int kAwBarriers = 4 * kAwSlots + 4 * kAwTiles + 1;
 constexpr int kAwInfo = 8;        // ints per slot
 constexpr int kAwSmemBytes = (kAwTiles + kAwSlots) * kFaTileBytes + 1024 + kAwSlots * (kFaRows + kAwInfo) * 4 +
                              kAwBarriers * 8 + 8 + (kAwSlots + kAwTiles) * 4;
-#ifndef QMOE_AW_POLY
-#define QMOE_AW_POLY 2
-#endif
-constexpr int kAwPoly = QMOE_AW_POLY;  // columns of 8 whose exp2 runs on the FMA pipe
 
 struct AttnWeightsArgs {
   const float* lse;
@@ -335,7 +331,6 @@ __global__ void __launch_bounds__(kAwThreads, 1)
     const int g = warp >> 2;
     const int r = (warp & 3) * 32 + lane;
     const uint32_t s_row = tmem_base + (uint32_t((warp & 3) * 32) << 16) + g * kFaRows;
-    const f32x2 scale2 = pack2(a.scale_log2, a.scale_log2);
     float total = 0.f;
     int uses = 0;
     for (int s = 0;; ++s) {
@@ -355,7 +350,6 @@ __global__ void __launch_bounds__(kAwThreads, 1)
         ++uses;
         tc_fence_after();
         float p8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        f32x2 sum2[2] = {0, 0};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           float v[32];
@@ -372,16 +366,7 @@ __global__ void __launch_bounds__(kAwThreads, 1)
               const float4 n4 = *reinterpret_cast<const float4*>(neg + c * 32 + e);
               const float nn[4] = {n4.x, n4.y, n4.z, n4.w};
 #pragma unroll
-              for (int k = 0; k < 4; k += 2) {
-                if (((e + k) & 7) < kAwPoly) {
-                  f32x2 p, q;
-                  exp2_poly2(fma2(pack2(v[e + k], v[e + k + 1]), scale2, pack2(nn[k], nn[k + 1])), p, q);
-                  sum2[(e >> 3) & 1] = fma2(p, q, sum2[(e >> 3) & 1]);
-                } else {
-                  p8[(e + k) & 7] += fa_exp2(fmaf(v[e + k], a.scale_log2, nn[k]));
-                  p8[(e + k + 1) & 7] += fa_exp2(fmaf(v[e + k + 1], a.scale_log2, nn[k + 1]));
-                }
-              }
+              for (int k = 0; k < 4; ++k) p8[(e + k) & 7] += fa_exp2(fmaf(v[e + k], a.scale_log2, nn[k]));
             }
           } else {
 #pragma unroll
@@ -392,9 +377,7 @@ __global__ void __launch_bounds__(kAwThreads, 1)
             }
           }
         }
-        float lo, hi;
-        unpack2(add2(sum2[0], sum2[1]), lo, hi);
-        total += (((p8[0] + p8[1]) + (p8[2] + p8[3])) + ((p8[4] + p8[5]) + (p8[6] + p8[7]))) + (lo + hi);
+        total += ((p8[0] + p8[1]) + (p8[2] + p8[3])) + ((p8[4] + p8[5]) + (p8[6] + p8[7]));
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&done[sl]);

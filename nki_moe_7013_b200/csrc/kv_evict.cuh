@@ -11,7 +11,7 @@
 // these few.
 //
 // kv_evict_select_kernel (one CTA per (sequence, KV head)) finds the n-th
-// largest of the 32-bit order keys digit by digit, lists the moves, and moves
+// largest of the 32-bit order keys eight bits at a time, lists the moves, and moves
 // the rows' weights and tokens; kv_evict_move_kernel copies the K and V rows
 // over all SMs and sets the new lengths.
 #pragma once
@@ -44,26 +44,29 @@ __device__ __forceinline__ uint32_t evict_key(float w, bool is_recent) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
+// Sum over the warps before this one, and over all (one value per warp in w).
+__device__ __forceinline__ int2 warps_before(const int* w, int warp, int warps, int lane) {
+  const int v = lane < warps ? w[lane] : 0;
+  return make_int2(__reduce_add_sync(0xFFFFFFFFu, lane < warp ? v : 0), __reduce_add_sync(0xFFFFFFFFu, v));
+}
+
 __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const EvictArgs a) {
   extern __shared__ uint32_t ev_keys[];
-  __shared__ int hist[256];
-  __shared__ int wsum[kEvWarps], wsum2[kEvWarps];
-  __shared__ int s_pick, s_rest, s_bad;
+  __shared__ int hist[2][256];
+  __shared__ int wsum[kEvWarps], wsum2[kEvWarps], wsum3[kEvWarps];
+  __shared__ int s_pick, s_rest, s_count;
   griddep_wait();
   griddep_launch_dependents();
   const int b = blockIdx.x / a.nkv, kvh = blockIdx.x % a.nkv;
+  const int threads = blockDim.x, warps = threads / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int32_t* plan = a.plan + size_t(blockIdx.x) * (2 + 2 * size_t(a.cap));
   int32_t* src = plan + 2;
   int32_t* dst = src + a.cap;
   int slot, lo, len;
   const bool ok = own_range(a.kv_len, a.cache_slot, a.kv_start, b, a.max_len, a.n_slots, slot, lo, len);
-  if (warp == 0) {
-    const bool dup = ok && slot_seen_before(a.cache_slot, b, lane);
-    if (lane == 0) s_bad = !ok || dup;
-  }
-  __syncthreads();
-  if (s_bad) {  // a bad length or slot, or a slot given twice: nothing of this entry changes
+  if (!ok || slot_seen_before(a.cache_slot, b, lane)) {
+    // a bad length or slot, or a slot given twice: nothing of this entry changes
     if (tid == 0) {
       record_device_error(kDevErrBadIndex);
       plan[0] = -1;
@@ -71,49 +74,56 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const Evict
     return;
   }
   const int n = min(a.keep, len - lo);
+  const bool all = n == len - lo;  // every live row stays
   float* w = a.weights + (size_t(slot) * a.nkv + kvh) * a.max_seq;
   int32_t* tok = a.tokens + (size_t(slot) * a.nkv + kvh) * a.max_seq;
 
   // the newest token
   int newest = INT32_MIN;
-  if (a.recent > 0) {
-    for (int r = lo + tid; r < len; r += kEvThreads) newest = max(newest, tok[r]);
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) newest = max(newest, __shfl_xor_sync(0xFFFFFFFFu, newest, off));
+  if (a.recent > 0 && !all) {
+#pragma unroll 4
+    for (int r = lo + tid; r < len; r += threads) newest = max(newest, tok[r]);
+    newest = __reduce_max_sync(0xFFFFFFFFu, newest);
     if (lane == 0) wsum[warp] = newest;
     __syncthreads();
-    newest = wsum[lane];
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) newest = max(newest, __shfl_xor_sync(0xFFFFFFFFu, newest, off));
+    newest = __reduce_max_sync(0xFFFFFFFFu, lane < warps ? wsum[lane] : INT32_MIN);
   }
   const long long old_most = (long long)newest - a.recent;  // tokens above it are recent
   auto fresh_key = [&](int r) { return evict_key(w[r], a.recent > 0 && (long long)tok[r] > old_most); };
-  for (int r = lo + tid; r < min(len, a.cached); r += kEvThreads) ev_keys[r] = fresh_key(r);
   auto key_at = [&](int r) { return r < a.cached ? ev_keys[r] : fresh_key(r); };
-  __syncthreads();
 
-  // the n-th largest key T: rows above T stay, and `take_eq` of those equal to it
+  // The n-th largest key T, eight bits at a time from the highest: rows above
+  // T stay, and `take_eq` of those equal to it.  A warp's equal digits are
+  // counted with one addition: the top digit is the exponent, which most rows
+  // share.
   uint32_t T = 0;
-  int take_eq = 0;
-  if (n == len - lo) {
-    take_eq = n;  // all stay (T = 0 lies below or at every key)
-  } else if (n > 0) {
-    uint32_t mask = 0;
-    int want = n;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      for (int r = lo + tid; r < len; r += kEvThreads) {
-        const uint32_t k = key_at(r);
-        if ((k & mask) == T) atomicAdd(&hist[(k >> shift) & 255], 1);
+  int take_eq = INT32_MAX;
+  if (!all && n > 0) {
+    for (int i = tid; i < 512; i += threads) hist[i >> 8][i & 255] = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int r0 = lo; r0 < len; r0 += threads) {
+      const int r = r0 + tid;
+      const bool live = r < len;
+      uint32_t k = 0;
+      if (live) {
+        k = fresh_key(r);
+        if (r < a.cached) ev_keys[r] = k;
       }
+      const uint32_t same = __match_any_sync(0xFFFFFFFFu, live ? k >> 24 : 256u);
+      if (live && lane == __ffs(same) - 1) atomicAdd(&hist[0][k >> 24], __popc(same));
+    }
+    uint32_t mask = 0xFF000000u;
+    int want = n;
+    for (int shift = 24, pass = 0;; shift -= 8, ++pass) {
       __syncthreads();
       if (warp == 0) {
         // lane i holds digits 255-8i .. 248-8i, largest first
+        const int* h = hist[pass & 1];
         int c[8], sum = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          c[e] = hist[255 - lane * 8 - e];
+          c[e] = h[255 - lane * 8 - e];
           sum += c[e];
         }
         int incl = sum;
@@ -129,56 +139,70 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const Evict
             if (above < want && want <= above + c[e]) {
               s_pick = 255 - lane * 8 - e;
               s_rest = want - above;
+              s_count = c[e];
             }
             above += c[e];
           }
         }
+      } else if (warp == 1) {
+        for (int i = lane; i < 256; i += 32) hist[(pass & 1) ^ 1][i] = 0;
       }
       __syncthreads();
       T |= uint32_t(s_pick) << shift;
       want = s_rest;
-      mask |= 0xFFu << shift;
+      if (want == s_count) break;  // every row with these digits stays: T's other digits are 0
+      if (shift == 0) {
+        take_eq = want;
+        break;
+      }
+      const int next = shift - 8;
+      int* h = hist[(pass & 1) ^ 1];
+      for (int r = lo + tid; r < len; r += threads) {
+        const uint32_t k = key_at(r);
+        if ((k & mask) == T) atomicAdd(&h[(k >> next) & 255], 1);
+      }
+      mask |= 0xFFu << next;
     }
-    take_eq = want;
-  } else {
-    T = 0xFFFFFFFFu;  // nothing stays
   }
-  const bool all = n == len - lo;
 
   // Each warp owns a contiguous run of rows, so ranks in row order are a scan
   // over the warps' totals plus ballots inside the run.
-  const int run = ((len + kEvWarps - 1) / kEvWarps + 31) / 32 * 32;
+  const int run = ((len + warps - 1) / warps + 31) / 32 * 32;
   const int r_begin = min(len, warp * run), r_end = min(len, r_begin + run);
-  int eq = 0;
-  for (int r0 = r_begin; r0 < r_end; r0 += 32) {
-    const int r = r0 + lane;
-    eq += __popc(__ballot_sync(0xFFFFFFFFu, r < r_end && r >= lo && key_at(r) == T));
-  }
-  if (lane == 0) wsum[warp] = eq;
-  __syncthreads();
+  const uint32_t before = (1u << lane) - 1u;
   int eq_before = 0;
-  for (int i = 0; i < warp; ++i) eq_before += wsum[i];
-  __syncthreads();
+  if (take_eq != INT32_MAX) {  // only then do equal rows need their rank
+    int eq = 0;
+    for (int r0 = r_begin; r0 < r_end; r0 += 32) {
+      const int r = r0 + lane;
+      eq += __popc(__ballot_sync(0xFFFFFFFFu, r < r_end && r >= lo && key_at(r) == T));
+    }
+    if (lane == 0) wsum3[warp] = eq;
+    __syncthreads();
+    eq_before = warps_before(wsum3, warp, warps, lane).x;
+  }
   // two passes: count the free rows below n and the kept rows beyond it, then list them
-  int holes_before = 0, moves_before = 0;
+  int holes_before = 0, moves_before = 0, n_moves = 0;
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
     int e = eq_before, holes = holes_before, moves = moves_before;
     for (int r0 = r_begin; r0 < r_end; r0 += 32) {
       const int r = r0 + lane;
       const bool live = r < r_end && r >= lo;
-      const uint32_t k = live ? key_at(r) : 0u;
-      const bool is_eq = live && k == T;
-      const uint32_t eqs = __ballot_sync(0xFFFFFFFFu, is_eq);
-      const uint32_t before = (1u << lane) - 1u;
-      const bool kept = live && (all || k > T || (is_eq && e + __popc(eqs & before) < take_eq));
-      const uint32_t hs = __ballot_sync(0xFFFFFFFFu, r < r_end && r < n && !kept);
-      const uint32_t ms = __ballot_sync(0xFFFFFFFFu, kept && r >= n);
-      if (pass == 1) {
-        if (r < r_end && r < n && !kept) dst[holes + __popc(hs & before)] = r;
-        if (kept && r >= n) src[moves + __popc(ms & before)] = r;
+      bool kept = live && all;
+      if (!all && n > 0) {
+        const uint32_t k = live ? key_at(r) : 0u;
+        const bool is_eq = live && k == T;
+        const uint32_t eqs = __ballot_sync(0xFFFFFFFFu, is_eq);
+        kept = live && (k > T || (is_eq && (take_eq == INT32_MAX || e + __popc(eqs & before) < take_eq)));
+        e += __popc(eqs);
       }
-      e += __popc(eqs);
+      const bool hole = r < r_end && r < n && !kept, move = kept && r >= n;
+      const uint32_t hs = __ballot_sync(0xFFFFFFFFu, hole), ms = __ballot_sync(0xFFFFFFFFu, move);
+      if (pass == 1) {
+        if (hole) dst[holes + __popc(hs & before)] = r;
+        if (move) src[moves + __popc(ms & before)] = r;
+      }
       holes += __popc(hs);
       moves += __popc(ms);
     }
@@ -188,30 +212,25 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const Evict
         wsum2[warp] = moves;
       }
       __syncthreads();
-      int total = 0;
-      for (int i = 0; i < kEvWarps; ++i) {
-        if (i < warp) {
-          holes_before += wsum[i];
-          moves_before += wsum2[i];
-        }
-        total += wsum2[i];
-      }
+      holes_before = warps_before(wsum, warp, warps, lane).x;
+      const int2 m = warps_before(wsum2, warp, warps, lane);
+      moves_before = m.x;
+      n_moves = m.y;
       if (tid == 0) {
-        plan[0] = total;
+        plan[0] = n_moves;
         plan[1] = n;
       }
     }
   }
-  int n_moves = 0;
-  for (int i = 0; i < kEvWarps; ++i) n_moves += wsum2[i];
   __syncthreads();
-  for (int i = tid; i < n_moves; i += kEvThreads) {
+  for (int i = tid; i < n_moves; i += threads) {
     const int s = src[i], d = dst[i];
     w[d] = w[s];
     tok[d] = tok[s];
   }
   __syncthreads();
-  for (int r = n + tid; r < len; r += kEvThreads) {
+#pragma unroll 4
+  for (int r = n + tid; r < len; r += threads) {
     w[r] = 0.f;
     tok[r] = -1;
   }

@@ -1851,7 +1851,10 @@ int qmoe_kv_evict(void* k_cache, void* v_cache, float* weights, int32_t* tokens,
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int smem = a.cached * 4;
   QMOE_CHECK(set_smem(qmoe::kv_evict_select_kernel, std::max(smem, 1024)));
-  QMOE_CHECK(launch_kernel(qmoe::kv_evict_select_kernel, dim3(unsigned(B * nkv)), dim3(qmoe::kEvThreads),
+  // about eight rows per thread: more threads only lengthen the barriers
+  int threads = 128;
+  while (threads < qmoe::kEvThreads && max_len > 8 * threads) threads *= 2;
+  QMOE_CHECK(launch_kernel(qmoe::kv_evict_select_kernel, dim3(unsigned(B * nkv)), dim3(unsigned(threads)),
                            size_t(smem), s, true, "kv_evict_select_kernel", a));
   const int64_t move_blocks = std::max<int64_t>(1, (a.cap + qmoe::kEvMoveRows - 1) / qmoe::kEvMoveRows);
   return launch_kernel(qmoe::kv_evict_move_kernel, dim3(unsigned(move_blocks), unsigned(B * nkv)), dim3(256), 0, s,
