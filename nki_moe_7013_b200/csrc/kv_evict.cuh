@@ -10,8 +10,9 @@
 // themselves, and an eviction of a few rows from a long cache moves only
 // these few.
 //
-// kv_evict_select_kernel (one CTA per (sequence, KV head)) finds the n-th
-// largest of the 32-bit order keys eight bits at a time, lists the moves, and moves
+// kv_evict_select_kernel (a cluster of one to eight CTAs per (sequence, KV
+// head), each holding a run of its rows) finds the n-th largest of the 32-bit
+// order keys eight bits at a time, lists the moves, and moves
 // the rows' weights and tokens; kv_evict_move_kernel copies the K and V rows
 // over all SMs and sets the new lengths.
 #pragma once
@@ -23,7 +24,8 @@ namespace qmoe {
 
 constexpr int kEvThreads = 1024;
 constexpr int kEvWarps = kEvThreads / 32;
-constexpr int kEvMaxCached = 49152;  // order keys held in shared memory (192 KB); rows past it are re-read from L2
+constexpr int kEvMaxCached = 32768;  // order keys a CTA holds in shared memory (128 KB); rows past it are re-read from L2
+constexpr int kEvMaxCluster = 8;
 constexpr int kEvMoveRows = 32;      // rows per CTA of the move kernel
 
 struct EvictArgs {
@@ -50,17 +52,49 @@ __device__ __forceinline__ int2 warps_before(const int* w, int warp, int warps, 
   return make_int2(__reduce_add_sync(0xFFFFFFFFu, lane < warp ? v : 0), __reduce_add_sync(0xFFFFFFFFu, v));
 }
 
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+// Barrier of the CTA, or of its whole cluster (shared and global memory).
+__device__ __forceinline__ void cluster_sync(int ranks) {
+  if (ranks == 1) {
+    __syncthreads();
+  } else {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+}
+// The word at p in the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ int ld_cluster(const int* p, int rank) {
+  uint32_t a;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+
 __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const EvictArgs a) {
-  extern __shared__ uint32_t ev_keys[];
-  __shared__ int hist[2][256];
-  __shared__ int wsum[kEvWarps], wsum2[kEvWarps], wsum3[kEvWarps];
+  extern __shared__ uint32_t ev_keys[];  // of this CTA's first a.cached rows
+  __shared__ int hist[2][256];           // read by the whole cluster
+  __shared__ int s_newest, s_eq, s_holes, s_moves;
+  __shared__ int hsum[256];
+  __shared__ int wsum[kEvWarps], wsum2[kEvWarps];
   __shared__ int s_pick, s_rest, s_count;
   griddep_wait();
   griddep_launch_dependents();
-  const int b = blockIdx.x / a.nkv, kvh = blockIdx.x % a.nkv;
+  const int rank = int(cluster_rank()), ranks = int(cluster_size());
+  const int unit = int(blockIdx.x) / ranks;
+  const int b = unit / a.nkv, kvh = unit % a.nkv;
   const int threads = blockDim.x, warps = threads / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int32_t* plan = a.plan + size_t(blockIdx.x) * (2 + 2 * size_t(a.cap));
+  int32_t* plan = a.plan + size_t(unit) * (2 + 2 * size_t(a.cap));
   int32_t* src = plan + 2;
   int32_t* dst = src + a.cap;
   int slot, lo, len;
@@ -77,20 +111,31 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const Evict
   const bool all = n == len - lo;  // every live row stays
   float* w = a.weights + (size_t(slot) * a.nkv + kvh) * a.max_seq;
   int32_t* tok = a.tokens + (size_t(slot) * a.nkv + kvh) * a.max_seq;
+  // this CTA's run of rows, and each warp's run within it: ranks in row order
+  // are sums over the CTAs and warps before, plus ballots inside the run
+  const int seg = ((len + ranks - 1) / ranks + 31) / 32 * 32;
+  const int s0 = min(len, rank * seg), s1 = min(len, s0 + seg);
+  const int run = ((s1 - s0 + warps - 1) / warps + 31) / 32 * 32;
+  const int r_begin = min(s1, s0 + warp * run), r_end = min(s1, r_begin + run);
 
   // the newest token
   int newest = INT32_MIN;
   if (a.recent > 0 && !all) {
 #pragma unroll 4
-    for (int r = lo + tid; r < len; r += threads) newest = max(newest, tok[r]);
+    for (int r = max(lo, s0) + tid; r < s1; r += threads) newest = max(newest, tok[r]);
     newest = __reduce_max_sync(0xFFFFFFFFu, newest);
     if (lane == 0) wsum[warp] = newest;
     __syncthreads();
     newest = __reduce_max_sync(0xFFFFFFFFu, lane < warps ? wsum[lane] : INT32_MIN);
+    if (ranks > 1) {
+      if (tid == 0) s_newest = newest;
+      cluster_sync(ranks);
+      newest = __reduce_max_sync(0xFFFFFFFFu, lane < ranks ? ld_cluster(&s_newest, lane) : INT32_MIN);
+    }
   }
   const long long old_most = (long long)newest - a.recent;  // tokens above it are recent
   auto fresh_key = [&](int r) { return evict_key(w[r], a.recent > 0 && (long long)tok[r] > old_most); };
-  auto key_at = [&](int r) { return r < a.cached ? ev_keys[r] : fresh_key(r); };
+  auto key_at = [&](int r) { return r - s0 < a.cached ? ev_keys[r - s0] : fresh_key(r); };
 
   // The n-th largest key T, eight bits at a time from the highest: rows above
   // T stay, and `take_eq` of those equal to it.  A warp's equal digits are
@@ -102,13 +147,13 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const Evict
     for (int i = tid; i < 512; i += threads) hist[i >> 8][i & 255] = 0;
     __syncthreads();
 #pragma unroll 4
-    for (int r0 = lo; r0 < len; r0 += threads) {
+    for (int r0 = s0; r0 < s1; r0 += threads) {
       const int r = r0 + tid;
-      const bool live = r < len;
+      const bool live = r >= lo && r < s1;
       uint32_t k = 0;
       if (live) {
         k = fresh_key(r);
-        if (r < a.cached) ev_keys[r] = k;
+        if (r - s0 < a.cached) ev_keys[r - s0] = k;
       }
       const uint32_t same = __match_any_sync(0xFFFFFFFFu, live ? k >> 24 : 256u);
       if (live && lane == __ffs(same) - 1) atomicAdd(&hist[0][k >> 24], __popc(same));
@@ -116,10 +161,22 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const Evict
     uint32_t mask = 0xFF000000u;
     int want = n;
     for (int shift = 24, pass = 0;; shift -= 8, ++pass) {
-      __syncthreads();
+      cluster_sync(ranks);  // the counts of this digit are there
+      const int* h = hist[pass & 1];
+      if (ranks > 1) {
+        for (int i = tid; i < 256; i += threads) {
+          int c[kEvMaxCluster], sum = 0;  // all loads in flight
+#pragma unroll
+          for (int k = 0; k < kEvMaxCluster; ++k) c[k] = k < ranks ? ld_cluster(h + i, k) : 0;
+#pragma unroll
+          for (int k = 0; k < kEvMaxCluster; ++k) sum += c[k];
+          hsum[i] = sum;
+        }
+        h = hsum;
+        __syncthreads();
+      }
       if (warp == 0) {
         // lane i holds digits 255-8i .. 248-8i, largest first
-        const int* h = hist[pass & 1];
         int c[8], sum = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -145,6 +202,7 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const Evict
           }
         }
       } else if (warp == 1) {
+        // (the cluster read these counts before its last barrier)
         for (int i = lane; i < 256; i += 32) hist[(pass & 1) ^ 1][i] = 0;
       }
       __syncthreads();
@@ -156,19 +214,16 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const Evict
         break;
       }
       const int next = shift - 8;
-      int* h = hist[(pass & 1) ^ 1];
-      for (int r = lo + tid; r < len; r += threads) {
+      int* hn = hist[(pass & 1) ^ 1];
+      for (int r = max(lo, s0) + tid; r < s1; r += threads) {
         const uint32_t k = key_at(r);
-        if ((k & mask) == T) atomicAdd(&h[(k >> next) & 255], 1);
+        if ((k & mask) == T) atomicAdd(&hn[(k >> next) & 255], 1);
       }
       mask |= 0xFFu << next;
     }
   }
+  __syncthreads();  // every thread's keys
 
-  // Each warp owns a contiguous run of rows, so ranks in row order are a scan
-  // over the warps' totals plus ballots inside the run.
-  const int run = ((len + warps - 1) / warps + 31) / 32 * 32;
-  const int r_begin = min(len, warp * run), r_end = min(len, r_begin + run);
   const uint32_t before = (1u << lane) - 1u;
   int eq_before = 0;
   if (take_eq != INT32_MAX) {  // only then do equal rows need their rank
@@ -177,9 +232,16 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const Evict
       const int r = r0 + lane;
       eq += __popc(__ballot_sync(0xFFFFFFFFu, r < r_end && r >= lo && key_at(r) == T));
     }
-    if (lane == 0) wsum3[warp] = eq;
+    if (lane == 0) wsum[warp] = eq;
     __syncthreads();
-    eq_before = warps_before(wsum3, warp, warps, lane).x;
+    const int2 e = warps_before(wsum, warp, warps, lane);
+    eq_before = e.x;
+    if (ranks > 1) {
+      if (tid == 0) s_eq = e.y;
+      cluster_sync(ranks);
+      eq_before += __reduce_add_sync(0xFFFFFFFFu, lane < rank ? ld_cluster(&s_eq, lane) : 0);
+    }
+    __syncthreads();
   }
   // two passes: count the free rows below n and the kept rows beyond it, then list them
   int holes_before = 0, moves_before = 0, n_moves = 0;
@@ -212,25 +274,37 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const Evict
         wsum2[warp] = moves;
       }
       __syncthreads();
-      holes_before = warps_before(wsum, warp, warps, lane).x;
-      const int2 m = warps_before(wsum2, warp, warps, lane);
+      const int2 h = warps_before(wsum, warp, warps, lane), m = warps_before(wsum2, warp, warps, lane);
+      holes_before = h.x;
       moves_before = m.x;
       n_moves = m.y;
-      if (tid == 0) {
+      if (ranks > 1) {
+        if (tid == 0) {
+          s_holes = h.y;
+          s_moves = m.y;
+        }
+        cluster_sync(ranks);
+        const int hk = lane < ranks ? ld_cluster(&s_holes, lane) : 0, mk = lane < ranks ? ld_cluster(&s_moves, lane) : 0;
+        holes_before += __reduce_add_sync(0xFFFFFFFFu, lane < rank ? hk : 0);
+        moves_before += __reduce_add_sync(0xFFFFFFFFu, lane < rank ? mk : 0);
+        n_moves = __reduce_add_sync(0xFFFFFFFFu, mk);
+      }
+      if (rank == 0 && tid == 0) {
         plan[0] = n_moves;
         plan[1] = n;
       }
     }
   }
-  __syncthreads();
-  for (int i = tid; i < n_moves; i += threads) {
+  cluster_sync(ranks);  // the lists are there
+  const int first = rank * threads + tid, step = ranks * threads;
+  for (int i = first; i < n_moves; i += step) {
     const int s = src[i], d = dst[i];
     w[d] = w[s];
     tok[d] = tok[s];
   }
-  __syncthreads();
+  cluster_sync(ranks);  // and the moved rows' weights and tokens were read
 #pragma unroll 4
-  for (int r = n + tid; r < len; r += threads) {
+  for (int r = n + first; r < len; r += step) {
     w[r] = 0.f;
     tok[r] = -1;
   }

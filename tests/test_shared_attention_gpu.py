@@ -374,7 +374,9 @@ EVICT = [
     ([1, 0], 2, [1500, 2000], [0, 700], 1024, 256),
     ([0], 2, [1031], None, 1030, 0),
     ([0], 2, [500], None, 0, 0),                     # nothing stays
-    ([0], 1, [50021], None, 20000, 1000),            # more rows than the select kernel holds in shared memory
+    ([0], 1, [50021], None, 20000, 1000),
+    ([1, 0], 2, [8200, 5000], [17, 0], 4100, 100),
+    ([0], 1, [270001], [3], 100000, 5000),           # more rows than the select kernel holds in shared memory
     ([0, 1], 1, [100, 90], [10, 0], 1000, 5),        # a budget over every length: paddings leave
 ]
 
