@@ -48,12 +48,13 @@ struct SharedDecodeArgs {
   float* pre_ml;    // [B*nh][psplits][2]
   float* own_o;     // own parts [own_cap][nh][128]
   float* own_ml;    // [own_cap][nh][2]
+  int2* plan;       // [B] a sequence's first own part and their number
   float* scores;    // [B*nkv][score_rows][G] log2-scaled scores of the own rows, or null
   float* weights;   // (n_slots, nkv, max_seq) or null
   __nv_bfloat16* out;
   int B, nh, nkv, G, max_seq, max_len, n_slots, accumulate;
   int P, prefix_z, psplits, pchunk, row_tiles, n_prefix_units;
-  int own_slots;    // parts per KV head that the own rows are cut into (at least one per sequence)
+  int own_slots;    // parts per KV head that the own rows are cut into (at least one per sequence); 0: one per sequence
   int n_own_units, score_rows, n_out_blocks, row_blocks;
   int direct;       // one unit per (sequence, KV head), nothing to join
   int overlaps;     // the kernel before it (the tcgen05 prefix part) may still run
@@ -75,28 +76,29 @@ __device__ __forceinline__ bool own_range(const int32_t* kv_len, const int32_t* 
   return ok;
 }
 
-// How the own rows of a batch are cut, found by every warp for itself: `chunk`
-// rows per part, and for sequence b its first part and their number.
-struct OwnParts {
-  int chunk, first, count;
-};
 __device__ __forceinline__ int own_rows(const SharedDecodeArgs& a, int b) {
   if (b >= a.B) return 0;
   int slot, lo, hi;
   own_range(a.kv_len, a.cache_slot, a.kv_start, b, a.max_len, a.n_slots, slot, lo, hi);
   return hi - lo;
 }
-// The parts of sequence b (part < 0), or the sequence that part `part` belongs
-// to (b out; B when there is no such part).
-__device__ __forceinline__ OwnParts own_parts(const SharedDecodeArgs& a, int& b, int part, int lane) {
+// How the own rows of a batch are cut, found by every warp for itself: `chunk`
+// rows per part, the sequence that part `part` belongs to (B when there is no
+// such part), and the sequence's first part and their number.
+struct OwnParts {
+  int b, chunk, first, count;
+};
+__device__ __forceinline__ OwnParts own_parts(const SharedDecodeArgs& a, int part, int lane) {
   const int first_rows = own_rows(a, lane);  // of the first 32 sequences: read once
   long long total = first_rows;
   for (int i = lane + 32; i < a.B; i += 32) total += own_rows(a, i);
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, off);
   OwnParts p;
-  const long long even = (total + a.own_slots - 1) / a.own_slots;
-  p.chunk = max(2 * kSdKeys, (int(min(even, (long long)a.max_len)) + kSdKeys - 1) / kSdKeys * kSdKeys);
+  const uint32_t rows = uint32_t(min(total, 0x7FFFFFFFll));  // (more are cut as if they were 2^31)
+  const int even = int(min((rows + a.own_slots - 1) / uint32_t(a.own_slots), uint32_t(a.max_len)));
+  p.chunk = max(2 * kSdKeys, (even + kSdKeys - 1) / kSdKeys * kSdKeys);
+  if (total > 0x7FFFFFFFll) p.chunk = max(p.chunk, (a.max_len + kSdKeys - 1) / kSdKeys * kSdKeys);
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 32) {
     const int n = ((b0 == 0 ? first_rows : own_rows(a, b0 + lane)) + p.chunk - 1) / p.chunk;
@@ -106,18 +108,17 @@ __device__ __forceinline__ OwnParts own_parts(const SharedDecodeArgs& a, int& b,
       const int t = __shfl_up_sync(0xFFFFFFFFu, incl, off);
       if (lane >= off) incl += t;
     }
-    const bool here = part < 0 ? b0 + lane == b : before + incl > part;
-    const uint32_t hit = __ballot_sync(0xFFFFFFFFu, here);
+    const uint32_t hit = __ballot_sync(0xFFFFFFFFu, before + incl > part);
     if (hit) {
       const int src = __ffs(hit) - 1;
-      if (part >= 0) b = b0 + src;
+      p.b = b0 + src;
       p.first = before + __shfl_sync(0xFFFFFFFFu, incl - n, src);
       p.count = __shfl_sync(0xFFFFFFFFu, n, src);
       return p;
     }
     before += __shfl_sync(0xFFFFFFFFu, incl, 31);
   }
-  b = a.B;
+  p.b = a.B;
   p.first = p.count = 0;
   return p;
 }
@@ -227,25 +228,22 @@ __global__ void __launch_bounds__(kSdThreads)
     const int v = u - a.n_prefix_units;
     kvh = v % a.nkv;
     part = v / a.nkv;
-    OwnParts parts = {};
-    if (a.direct)
-      own_b = part;
-    else
-      parts = own_parts(a, own_b, part, lane);
+    const bool whole = a.own_slots == 0;  // a sequence is one part (and with `direct` the only one)
+    OwnParts parts = {part, 0, part, 1};
+    if (!whole) parts = own_parts(a, part, lane);
+    own_b = parts.b;
     live = own_b < a.B;  // there may be fewer parts than units
     if (live) {
       int hi;
       if (!own_range(a.kv_len, a.cache_slot, a.kv_start, own_b, a.max_len, a.n_slots, slot, lo, hi) &&
           threadIdx.x == 0)
         record_device_error(kDevErrBadIndex);
-      if (a.direct) {
+      k0 = whole ? lo : lo + (part - parts.first) * parts.chunk;
+      k1 = whole ? hi : min(hi, k0 + parts.chunk);
+      if (a.direct)
         p1 = a.P;
-        k0 = lo;
-        k1 = hi;
-      } else {
-        k0 = lo + (part - parts.first) * parts.chunk;
-        k1 = min(hi, k0 + parts.chunk);
-      }
+      else if (kvh == 0 && part == parts.first && threadIdx.x == 0)
+        a.plan[own_b] = make_int2(parts.first, k1 > k0 ? parts.count : 0);
     }
     row0 = own_b * a.G;
     n_rows = a.G;
@@ -509,10 +507,16 @@ struct RowParts {
                                             lane * 4);
   }
 };
-__device__ __forceinline__ RowParts row_parts(const SharedDecodeArgs& a, const OwnParts& own, int b, int h) {
-  const size_t bh = size_t(b) * a.nh + h, first = size_t(own.first) * a.nh + h;
+// (A sequence without own rows has no part that wrote its plan.)
+__device__ __forceinline__ RowParts row_parts(const SharedDecodeArgs& a, int own_count, int own_first, int b, int h) {
+  const size_t bh = size_t(b) * a.nh + h, first = size_t(own_first) * a.nh + h;
   return {a.pre_ml + bh * a.psplits * 2, a.pre_o + bh * a.psplits * kAttnD, a.own_ml + first * 2,
-          a.own_o + first * kAttnD,      a.psplits, a.psplits + own.count,  a.nh};
+          a.own_o + first * kAttnD,      a.psplits, a.psplits + own_count,  a.nh};
+}
+__device__ __forceinline__ int2 own_plan(const SharedDecodeArgs& a, int b) {
+  if (a.max_len == 0) return make_int2(0, 0);
+  const int2 p = a.plan[b];
+  return own_rows(a, b) > 0 ? p : make_int2(0, 0);
 }
 
 // M and 1/l of one row from its parts, in every lane of the warp.
@@ -547,9 +551,9 @@ __global__ void __launch_bounds__(256) shared_decode_combine_kernel(const Shared
   if (int(blockIdx.x) < a.n_out_blocks) {
     const int gw = blockIdx.x * 8 + warp;
     if (gw >= a.B * a.nh) return;
-    int b = gw / a.nh;
-    const OwnParts own = own_parts(a, b, -1, lane);
-    const RowParts p = row_parts(a, own, b, gw % a.nh);
+    const int b = gw / a.nh;
+    const int2 own = own_plan(a, b);
+    const RowParts p = row_parts(a, own.y, own.x, b, gw % a.nh);
     float M, inv;
     join_ml(p, lane, M, inv);
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -562,14 +566,13 @@ __global__ void __launch_bounds__(256) shared_decode_combine_kernel(const Shared
         v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (s0 + j < p.n) {
           const float2 ml = p.ml(s0 + j);
-          if (ml.y != 0.f) {  // an empty part has no output
-            sc[j] = exp2f(ml.x - M);
-            v[j] = p.o(s0 + j, lane);
-          }
+          v[j] = p.o(s0 + j, lane);
+          if (ml.y != 0.f) sc[j] = exp2f(ml.x - M);
         }
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
+        if (sc[j] == 0.f) continue;  // an empty part has no output; one so small adds nothing
         acc[0] += v[j].x * sc[j];
         acc[1] += v[j].y * sc[j];
         acc[2] += v[j].z * sc[j];
@@ -584,16 +587,23 @@ __global__ void __launch_bounds__(256) shared_decode_combine_kernel(const Shared
   }
   const int v = blockIdx.x - a.n_out_blocks;
   const int rb = v % a.row_blocks, rest = v / a.row_blocks;
-  const int kvh = rest % a.nkv;
-  int b = rest / a.nkv;
+  const int kvh = rest % a.nkv, b = rest / a.nkv;
   int slot, lo, hi;
   if (!own_range(a.kv_len, a.cache_slot, a.kv_start, b, a.max_len, a.n_slots, slot, lo, hi)) return;  // recorded before
   const int first = rb * kSdCombineRows;
   if (first >= hi) return;
-  const OwnParts own = own_parts(a, b, -1, lane);
+  const int row = first + threadIdx.x;
+  // the row's scores and total, in flight while the maxima are joined
+  const float* sp = a.scores + (size_t(b * a.nkv + kvh) * a.score_rows + row) * a.G;
+  float* dst = a.weights + (size_t(slot) * a.nkv + kvh) * a.max_seq + row;
+  float sc[kSdMaxGroup];
+#pragma unroll
+  for (int h = 0; h < kSdMaxGroup; ++h) sc[h] = h < a.G && row >= lo && row < hi ? sp[h] : -INFINITY;
+  const float total = a.accumulate && row < hi ? *dst : 0.f;
+  const int2 own = own_plan(a, b);
   for (int h = warp; h < a.G; h += 8) {
     float M, inv;
-    join_ml(row_parts(a, own, b, kvh * a.G + h), lane, M, inv);
+    join_ml(row_parts(a, own.y, own.x, b, kvh * a.G + h), lane, M, inv);
     if (lane == 0) {
       sM[h] = M;
       sInv[h] = inv;
@@ -608,15 +618,12 @@ __global__ void __launch_bounds__(256) shared_decode_combine_kernel(const Shared
     }
   }
   __syncthreads();
-  const int row = first + threadIdx.x;
   if (s_dup || row >= hi) return;
   float w = 0.f;
-  if (row >= lo) {
-    const float* sc = a.scores + (size_t(b * a.nkv + kvh) * a.score_rows + row) * a.G;
-    for (int h = 0; h < a.G; ++h) w += exp2f(sc[h] - sM[h]) * sInv[h];
-  }
-  float* dst = a.weights + (size_t(slot) * a.nkv + kvh) * a.max_seq + row;
-  *dst = a.accumulate ? *dst + w : w;
+#pragma unroll
+  for (int h = 0; h < kSdMaxGroup; ++h)
+    if (h < a.G && row >= lo) w += exp2f(sc[h] - sM[h]) * sInv[h];
+  *dst = total + w;
 }
 
 }  // namespace qmoe

@@ -457,13 +457,31 @@ __global__ void __launch_bounds__(kFaThreads, 1)
           tmem_ld_x32(o_col + c * 32, ov);
           tmem_ld_wait();
         }
-        if (!mine) continue;
         if constexpr (kPartial) {
-          float4* dst = reinterpret_cast<float4*>(a.part_o + (row * a.nparts + part) * kFaD) + c * 8;
+          // through this warp's 4 KB of the group's P tile, so that a store
+          // covers whole 128-byte lines of four rows
+          const uint32_t stage = smem_u32(sP + g * kFaTileBytes) + quad * 4096;
 #pragma unroll
           for (int q = 0; q < 8; ++q)
-            dst[q] = make_float4(ov[q * 4], ov[q * 4 + 1], ov[q * 4 + 2], ov[q * 4 + 3]);
-        } else {
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + ((q ^ (lane & 7)) << 4)),
+                         "f"(ov[q * 4]), "f"(ov[q * 4 + 1]), "f"(ov[q * 4 + 2]), "f"(ov[q * 4 + 3])
+                         : "memory");
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const int rr = q * 4 + (lane >> 3), ch = lane & 7;  // row of the warp, 16-byte chunk
+            float4 v;
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                         : "r"(stage + rr * 128 + ((ch ^ (rr & 7)) << 4)));
+            const int tr = quad * 32 + rr, rq = q0 + (kSplit ? 0 : g * per_q) + tr / a.G;
+            if (tr < tile_rows && rq < a.B) {
+              const size_t at = size_t(rq) * a.nh + kvh * a.G + tr % a.G;
+              *(reinterpret_cast<float4*>(a.part_o + (at * a.nparts + part) * kFaD) + c * 8 + ch) = v;
+            }
+          }
+          __syncwarp();
+        } else if (mine) {
           uint4* dst = reinterpret_cast<uint4*>(a.out + row * kFaD) + c * 4;
 #pragma unroll
           for (int q = 0; q < 4; ++q)

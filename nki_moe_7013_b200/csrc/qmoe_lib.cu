@@ -956,7 +956,7 @@ struct SharedDecodePlan {
 };
 
 // Rows (prefix and own) up to which a sequence's keys are not cut.
-constexpr int64_t kDirectRows = 512;
+constexpr int64_t kDirectRows = 256;
 
 // Rows (sequences x heads of a group) above which the prefix part runs on the
 // tcgen05 kernel.
@@ -996,9 +996,10 @@ SharedDecodePlan shared_decode_plan(int64_t B, int64_t G, int64_t nkv, int64_t P
     p.psplits = (P + p.pchunk - 1) / p.pchunk;
   }
   if (max_len > 0) {
-    // two CTAs per SM; every sequence has a part of its own, none shorter than 128 rows but its last
-    p.own_slots = std::max<int64_t>(1, 2 * sms / nkv);
-    p.own_cap = std::min(p.own_slots + B, B * ((max_len + 127) / 128));
+    // two CTAs per SM; every sequence has a part of its own, none shorter than
+    // 128 rows but its last.  Sequences that fill the SMs are not cut.
+    p.own_slots = B * nkv >= 2 * sms ? 0 : std::max<int64_t>(1, 2 * sms / nkv);
+    p.own_cap = p.own_slots == 0 ? B : std::min(p.own_slots + B, B * ((max_len + 127) / 128));
   }
   return p;
 }
@@ -1587,7 +1588,7 @@ size_t qmoe_attention_prefix_decode_workspace_size(int64_t B, int64_t nh, int64_
   if (B <= 0 || nkv <= 0 || nh <= 0 || nh % nkv != 0 || prefix_len < 0 || max_len < 0) return 0;
   const SharedDecodePlan p = shared_decode_plan(B, nh / nkv, nkv, prefix_len, max_len);
   const size_t rows = size_t(B * nh * p.psplits + p.own_cap * nh);
-  return (rows * (qmoe::kAttnD + 2) + (with_weights ? size_t(B * nh) * size_t(max_len) : 0)) * sizeof(float) + 256;
+  return size_t(B) * sizeof(int2) + (rows * (qmoe::kAttnD + 2) + (with_weights ? size_t(B * nh) * size_t(max_len) : 0)) * sizeof(float) + 256;
 }
 
 int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void* v_prefix, int64_t n_prefix_slots,
@@ -1620,7 +1621,8 @@ int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void
   a.own_o = a.pre_o + size_t(B * nh * p.psplits) * qmoe::kAttnD;
   a.pre_ml = a.own_o + size_t(p.own_cap * nh) * qmoe::kAttnD;
   a.own_ml = a.pre_ml + size_t(B * nh * p.psplits) * 2;
-  a.scores = weights ? a.own_ml + size_t(p.own_cap * nh) * 2 : nullptr;
+  a.plan = reinterpret_cast<int2*>(a.own_ml + size_t(p.own_cap * nh) * 2);
+  a.scores = weights ? reinterpret_cast<float*>(a.plan + B) : nullptr;
   CUtensorMap tk, tv, tkp, tvp;
   QMOE_CHECK(make_tmap_rows(&tk, k_cache, max_seq, max_seq, n_slots * nkv, qmoe::kSdKeys));
   QMOE_CHECK(make_tmap_rows(&tv, v_cache, max_seq, max_seq, n_slots * nkv, qmoe::kSdKeys));
