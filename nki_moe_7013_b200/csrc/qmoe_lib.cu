@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -165,6 +166,20 @@ static int set_smem(Kernel k, int bytes) {
   if (err != cudaSuccess)
     return set_error(QMOE_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(err));
   return QMOE_OK;
+}
+
+// set_smem once per kernel and device (the attribute stays with the kernel).
+template <auto kKernel>
+static int set_smem_once(int bytes) {
+  static std::atomic<uint64_t> done{0};  // bit per device
+  static_assert(kMaxDevices <= 64, "one bit per device");
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices &&
+      (done.load(std::memory_order_relaxed) >> dev & 1))
+    return QMOE_OK;
+  const int st = set_smem(kKernel, bytes);
+  if (st == QMOE_OK && dev >= 0 && dev < kMaxDevices) done.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+  return st;
 }
 
 // Kernel launch through cudaLaunchKernelEx; with `pdl` the launch allows
@@ -929,11 +944,18 @@ int make_tmap_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t str
 int launch_flash_prefix(bool partial, bool split, int64_t ctas, const CUtensorMap& tq, const CUtensorMap& tk,
                         const CUtensorMap& tv, const CUtensorMap& tkp, const CUtensorMap& tvp,
                         const qmoe::FlashPrefixArgs& a, cudaStream_t s) {
-  auto* kernel = partial ? (split ? qmoe::flash_prefix_kernel<true, true> : qmoe::flash_prefix_kernel<true, false>)
-                         : (split ? qmoe::flash_prefix_kernel<false, true> : qmoe::flash_prefix_kernel<false, false>);
-  QMOE_CHECK(set_smem(kernel, qmoe::kFpSmemBytes));
-  return launch_kernel(kernel, dim3(unsigned(ctas)), dim3(qmoe::kFaThreads), size_t(qmoe::kFpSmemBytes), s, true,
-                       "flash_prefix_kernel", tq, tk, tv, tkp, tvp, a);
+#define QMOE_FLASH_PREFIX(P, S)                                                                                      \
+  if (partial == P && split == S) {                                                                                  \
+    QMOE_CHECK((set_smem_once<qmoe::flash_prefix_kernel<P, S>>(qmoe::kFpSmemBytes)));                                 \
+    return launch_kernel(qmoe::flash_prefix_kernel<P, S>, dim3(unsigned(ctas)), dim3(qmoe::kFaThreads),               \
+                         size_t(qmoe::kFpSmemBytes), s, true, "flash_prefix_kernel", tq, tk, tv, tkp, tvp, a);       \
+  }
+  QMOE_FLASH_PREFIX(true, true)
+  QMOE_FLASH_PREFIX(true, false)
+  QMOE_FLASH_PREFIX(false, true)
+  QMOE_FLASH_PREFIX(false, false)
+#undef QMOE_FLASH_PREFIX
+  return QMOE_OK;  // not reached
 }
 
 // Row tiles of flash_prefix_kernel: a CTA takes two that share its key tiles,
@@ -1588,7 +1610,8 @@ size_t qmoe_attention_prefix_decode_workspace_size(int64_t B, int64_t nh, int64_
   if (B <= 0 || nkv <= 0 || nh <= 0 || nh % nkv != 0 || prefix_len < 0 || max_len < 0) return 0;
   const SharedDecodePlan p = shared_decode_plan(B, nh / nkv, nkv, prefix_len, max_len);
   const size_t rows = size_t(B * nh * p.psplits + p.own_cap * nh);
-  return size_t(B) * sizeof(int2) + (rows * (qmoe::kAttnD + 2) + (with_weights ? size_t(B * nh) * size_t(max_len) : 0)) * sizeof(float) + 256;
+  const size_t scores = with_weights ? size_t(B * nh) * size_t(max_len) * sizeof(float) : 0;
+  return p.direct ? scores : rows * (qmoe::kAttnD + 2) * sizeof(float) + size_t(B) * sizeof(int2) + scores;
 }
 
 int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void* v_prefix, int64_t n_prefix_slots,
@@ -1597,16 +1620,18 @@ int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void
                                  const int32_t* kv_start, int64_t B, int64_t nh, int64_t nkv, int64_t head_dim,
                                  int64_t n_slots, int64_t max_seq, int64_t max_len, float scale, float* weights,
                                  int accumulate, void* out, void* workspace, size_t workspace_bytes, void* stream) {
-  QMOE_REQUIRE(q && k_cache && v_cache && kv_len && out && workspace, QMOE_ERR_INVALID_ARGUMENT,
+  QMOE_REQUIRE(q && k_cache && v_cache && kv_len && out, QMOE_ERR_INVALID_ARGUMENT,
                "attention_prefix_decode: null pointer");
   QMOE_CHECK(check_shared_attention("attention_prefix_decode", head_dim, nh, nkv, n_slots, max_seq, scale));
   QMOE_CHECK(check_prefix("attention_prefix_decode", k_prefix, v_prefix, n_prefix_slots, prefix_max, prefix_slot,
                           prefix_len, nkv));
   QMOE_REQUIRE(B >= 0 && B <= 65535 && max_len >= 0 && max_len <= max_seq && (cache_slot || B <= n_slots),
                QMOE_ERR_INVALID_ARGUMENT, "attention_prefix_decode: bad sizes");
-  QMOE_REQUIRE(workspace_bytes >= qmoe_attention_prefix_decode_workspace_size(B, nh, nkv, prefix_len, max_len,
-                                                                              weights != nullptr),
-               QMOE_ERR_WORKSPACE_TOO_SMALL, "attention_prefix_decode: workspace too small");
+  const size_t need =
+      qmoe_attention_prefix_decode_workspace_size(B, nh, nkv, prefix_len, max_len, weights != nullptr);
+  QMOE_REQUIRE(workspace || need == 0, QMOE_ERR_INVALID_ARGUMENT, "attention_prefix_decode: null workspace");
+  QMOE_REQUIRE(workspace_bytes >= need, QMOE_ERR_WORKSPACE_TOO_SMALL,
+               "attention_prefix_decode: workspace too small");
   QMOE_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out) &&
                    (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
                QMOE_ERR_MISALIGNED, "attention_prefix_decode: pointers must be 16-byte aligned (workspace 256)");
@@ -1622,7 +1647,7 @@ int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void
   a.pre_ml = a.own_o + size_t(p.own_cap * nh) * qmoe::kAttnD;
   a.own_ml = a.pre_ml + size_t(B * nh * p.psplits) * 2;
   a.plan = reinterpret_cast<int2*>(a.own_ml + size_t(p.own_cap * nh) * 2);
-  a.scores = weights ? reinterpret_cast<float*>(a.plan + B) : nullptr;
+  a.scores = !weights ? nullptr : p.direct ? static_cast<float*>(workspace) : reinterpret_cast<float*>(a.plan + B);
   CUtensorMap tk, tv, tkp, tvp;
   QMOE_CHECK(make_tmap_rows(&tk, k_cache, max_seq, max_seq, n_slots * nkv, qmoe::kSdKeys));
   QMOE_CHECK(make_tmap_rows(&tv, v_cache, max_seq, max_seq, n_slots * nkv, qmoe::kSdKeys));
@@ -1682,7 +1707,7 @@ int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void
   a.scale_log2 = scale * 1.4426950408889634f;
   const int64_t units = int64_t(a.n_prefix_units) + a.n_own_units;
   if (units > 0) {
-    QMOE_CHECK(set_smem(qmoe::shared_decode_kernel, qmoe::kSdSmemBytes));
+    QMOE_CHECK(set_smem_once<qmoe::shared_decode_kernel>(qmoe::kSdSmemBytes));
     QMOE_CHECK(launch_kernel(qmoe::shared_decode_kernel, dim3(unsigned(units)), dim3(qmoe::kSdThreads),
                              size_t(qmoe::kSdSmemBytes), s, true, "shared_decode_kernel", tk, tv, tkp, tvp, a));
   }
@@ -1774,8 +1799,9 @@ int qmoe_attention_weights(const void* q, const float* lse, const void* k_cache,
   const int64_t units = p.chunks * B * nkv * p.key_blocks;
   QMOE_REQUIRE(B * S < (int64_t(1) << 30) && units < (int64_t(1) << 30), QMOE_ERR_INVALID_ARGUMENT,
                "attention_weights: too many queries");
-  QMOE_REQUIRE(workspace_bytes >= qmoe_attention_weights_workspace_size(B, S, nh, nkv, max_len),
-               QMOE_ERR_WORKSPACE_TOO_SMALL, "attention_weights: workspace too small");
+  const size_t need = qmoe_attention_weights_workspace_size(B, S, nh, nkv, max_len);
+  QMOE_REQUIRE(workspace || need == 0, QMOE_ERR_INVALID_ARGUMENT, "attention_weights: null workspace");
+  QMOE_REQUIRE(workspace_bytes >= need, QMOE_ERR_WORKSPACE_TOO_SMALL, "attention_weights: workspace too small");
   CUtensorMap tq, tk;
   QMOE_CHECK(make_tmap_bf16_3d(&tq, q, 128, uint64_t(nh), uint64_t(B * S), 256, uint64_t(nh) * 256, 64, uint32_t(G),
                                uint32_t(qmoe::kFaRows / G)));
@@ -1801,7 +1827,7 @@ int qmoe_attention_weights(const void* q, const float* lse, const void* k_cache,
   a.chunk = int(p.chunk);
   a.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  QMOE_CHECK(set_smem(qmoe::attn_weights_kernel, qmoe::kAwSmemBytes));
+  QMOE_CHECK(set_smem_once<qmoe::attn_weights_kernel>(qmoe::kAwSmemBytes));
   QMOE_CHECK(launch_kernel(qmoe::attn_weights_kernel, dim3(unsigned(std::min<int64_t>(units, d->sms))),
                            dim3(qmoe::kAwThreads), size_t(qmoe::kAwSmemBytes), s, true, "attn_weights_kernel", tq, tk,
                            a));
@@ -1860,7 +1886,7 @@ int qmoe_kv_evict(void* k_cache, void* v_cache, float* weights, int32_t* tokens,
   while (threads < qmoe::kEvThreads && max_len > 4 * threads * cluster) threads *= 2;
   a.cached = int(std::min<int64_t>(((max_len + cluster - 1) / cluster + 31) / 32 * 32, qmoe::kEvMaxCached));
   const int smem = a.cached * 4;
-  QMOE_CHECK(set_smem(qmoe::kv_evict_select_kernel, std::max(smem, 1024)));
+  QMOE_CHECK(set_smem_once<qmoe::kv_evict_select_kernel>(qmoe::kEvMaxCached * 4));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(B * nkv * cluster));
   cfg.blockDim = dim3(unsigned(threads));

@@ -638,18 +638,29 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 # shared prefixes and bounded caches
 # ----------------------------------------------------------------------------
 
-def _launch(dev: torch.device, what: str, fn, *args) -> None:
-    """fn(*args, stream) with ``dev`` current, on its current stream.  (The
+_BF16, _F32, _I32, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
+
+
+def _launch(i: int, what: str, fn, *args) -> None:
+    """fn(*args, stream) with device ``i`` current, on its current stream.  (The
     device guard and the stream object cost 4 us of host time per call, which
     a call of a few rows would wait for; both are skipped where they can be.)"""
-    i = dev.index
     if torch._C._cuda_getDevice() == i:
         st = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(i):
             st = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     if st != 0:
         _C.check(st, what)
+
+
+def _plain(i: int, dtype, *tensors) -> bool:
+    """Every tensor given (None: skipped) is contiguous, of ``dtype`` and on
+    device ``i``: the quick look that spares a good call the named checks."""
+    for t in tensors:
+        if t is not None and not (t.dtype is dtype and t.get_device() == i and t.is_contiguous()):
+            return False
+    return True
 
 
 def _need_rows(t: torch.Tensor, name: str, dtype, k_cache: torch.Tensor):
@@ -678,16 +689,15 @@ def _need_i32(t: Optional[torch.Tensor], name: str, n: int, dev):
 
 
 def _need_prefix(k_prefix, v_prefix, prefix_len: int, k_cache: torch.Tensor):
-    """(pointer, pointer, slots, rows per slot) of a prefix; nulls without one."""
+    """A prefix of prefix_len rows that goes with the cache."""
     if prefix_len == 0:
-        return None, None, 0, 0
+        return
     if k_prefix is None or v_prefix is None:
         raise ValueError("a prefix of more than 0 rows needs k_prefix and v_prefix")
     _need_cache(k_prefix, v_prefix, "prefix")
-    n, nkv, rows, hd = k_prefix.shape
-    if nkv != k_cache.shape[1] or hd != k_cache.shape[3] or k_prefix.device != k_cache.device:
+    if k_prefix.shape[1] != k_cache.shape[1] or k_prefix.shape[3] != k_cache.shape[3] or \
+            k_prefix.device != k_cache.device:
         raise ValueError("the prefix must have the cache's KV heads, head dim and device")
-    return k_prefix.data_ptr(), v_prefix.data_ptr(), n, rows
 
 
 def _need_heads(q: torch.Tensor, rows: int, k_cache: torch.Tensor):
@@ -714,14 +724,45 @@ def _weights_bytes(device: int, B: int, S: int, nh: int, nkv: int, max_len: int)
         return int(_C.lib().qmoe_attention_weights_workspace_size(B, S, nh, nkv, max_len))
 
 
-def _workspace(given: Optional[torch.Tensor], nbytes: int, dev) -> torch.Tensor:
+def _workspace(given: Optional[torch.Tensor], nbytes: int, like: torch.Tensor):
+    """(pointer, bytes) of a workspace: the caller's if it is large enough, a
+    new one, or none where none is needed; and the tensor that holds it."""
     if given is not None:
-        _need(given, "workspace", torch.uint8, 1)
-        if given.device != dev:
-            raise ValueError(f"workspace must be on {dev}")
+        _need(given, "workspace", _U8, 1)
+        if given.device != like.device:
+            raise ValueError(f"workspace must be on {like.device}")
         if given.shape[0] >= nbytes:
-            return given
-    return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+            return given.data_ptr(), given.shape[0], given
+    if nbytes == 0:
+        return None, 0, None
+    ws = like.new_empty(nbytes, dtype=_U8)
+    return ws.data_ptr(), nbytes, ws
+
+
+def _need_decode(q, k_prefix, v_prefix, prefix_len, k_cache, v_cache, kv_len, cache_slot, kv_start, weights):
+    """The named checks of attention_prefix_decode."""
+    _need_cache(k_cache, v_cache)
+    _need(kv_len, "kv_len", _I32, 1)
+    B, dev = kv_len.shape[0], k_cache.device
+    _need_heads(q, B, k_cache)
+    _need_i32(kv_len, "kv_len", B, dev)
+    _need_i32(cache_slot, "cache_slot", B, dev)
+    _need_i32(kv_start, "kv_start", B, dev)
+    _need_batch(B, cache_slot, k_cache)
+    _need_prefix(k_prefix, v_prefix, prefix_len, k_cache)
+    if weights is not None:
+        _need_rows(weights, "weights", _F32, k_cache)
+
+
+def _need_queries(q, B, S, k_cache, q_start, cache_slot, kv_start):
+    """The named checks that attention_prefix_prefill and attention_weights share."""
+    _need_heads(q, B * S, k_cache)
+    dev = k_cache.device
+    _need(q_start, "q_start", _I32, 1)
+    _need_i32(q_start, "q_start", B, dev)
+    _need_i32(cache_slot, "cache_slot", B, dev)
+    _need_i32(kv_start, "kv_start", B, dev)
+    _need_batch(B, cache_slot, k_cache)
 
 
 def attention_prefix_decode(q: torch.Tensor, k_prefix: Optional[torch.Tensor], v_prefix: Optional[torch.Tensor],
@@ -738,30 +779,38 @@ def attention_prefix_decode(q: torch.Tensor, k_prefix: Optional[torch.Tensor], v
     ``weights`` (n_slots, nkv, max_seq) fp32: every own row's attention
     probability, summed over the query heads of its KV head, is added to it
     (``accumulate=False``: replaces it)."""
-    _need_cache(k_cache, v_cache)
-    _need(kv_len, "kv_len", torch.int32, 1)
-    B = kv_len.shape[0]
-    _need_heads(q, B, k_cache)
-    nh, hd = q.shape[1], q.shape[2]
-    dev = k_cache.device
-    _need_i32(kv_len, "kv_len", B, dev)
-    _need_i32(cache_slot, "cache_slot", B, dev)
-    _need_i32(kv_start, "kv_start", B, dev)
-    _need_batch(B, cache_slot, k_cache)
-    kp, vp, n_prefix, prefix_max = _need_prefix(k_prefix, v_prefix, prefix_len, k_cache)
-    if weights is not None:
-        _need_rows(weights, "weights", torch.float32, k_cache)
-    n_slots, nkv, max_seq, _ = k_cache.shape
-    out = torch.empty((B, nh * hd), dtype=torch.bfloat16, device=dev)
+    try:
+        i = k_cache.get_device()
+        n_slots, nkv, max_seq, hd = rows = k_cache.shape
+        B, nh, d = q.shape
+        if prefix_len:
+            n_prefix, pkv, prefix_max, pd = pshape = k_prefix.shape
+        good = (i >= 0 and d == hd and _plain(i, _BF16, q, k_cache, v_cache)
+                and _plain(i, _I32, kv_len, cache_slot, kv_start) and v_cache.shape == rows
+                and kv_len.shape == (B,) and (B <= n_slots if cache_slot is None else cache_slot.shape == (B,))
+                and (kv_start is None or kv_start.shape == (B,))
+                and (not prefix_len or (_plain(i, _BF16, k_prefix, v_prefix) and v_prefix.shape == pshape
+                                        and pkv == nkv and pd == hd))
+                and (weights is None or (_plain(i, _F32, weights) and weights.shape == rows[:3])))
+    except (AttributeError, ValueError):
+        good = False
+    if not good:
+        _need_decode(q, k_prefix, v_prefix, prefix_len, k_cache, v_cache, kv_len, cache_slot, kv_start, weights)
+    out = q.new_empty((B, nh * hd))
     if B == 0:
         return out
-    ws = _workspace(workspace, _prefix_decode_bytes(dev.index, B, nh, nkv, prefix_len, max_len,
-                                                    0 if weights is None else 1), dev)
-    _launch(dev, "qmoe_attention_prefix_decode", _C.lib().qmoe_attention_prefix_decode,
+    if prefix_len:
+        kp, vp = k_prefix.data_ptr(), v_prefix.data_ptr()
+    else:
+        kp = vp = None
+        n_prefix = prefix_max = 0
+    w, nbytes, _ws = _workspace(workspace, _prefix_decode_bytes(i, B, nh, nkv, prefix_len, max_len,
+                                                                0 if weights is None else 1), q)
+    _launch(i, "qmoe_attention_prefix_decode", _C.lib().qmoe_attention_prefix_decode,
             q.data_ptr(), kp, vp, n_prefix, prefix_max, prefix_slot, prefix_len, k_cache.data_ptr(),
             v_cache.data_ptr(), kv_len.data_ptr(), _ptr(cache_slot), _ptr(kv_start), B, nh, nkv, hd, n_slots, max_seq,
             max_len, hd ** -0.5 if scale is None else scale, _ptr(weights), 1 if accumulate else 0, out.data_ptr(),
-            ws.data_ptr(), ws.shape[0])
+            w, nbytes)
     return out
 
 
@@ -800,21 +849,33 @@ def attention_prefix_prefill(q: torch.Tensor, k_prefix: Optional[torch.Tensor], 
     query before kv_start (padding) gets zeros.  With ``return_lse`` also the
     log-sum-exp (B*S, nh) fp32 of each row's scores (-inf for padding), which
     attention_weights takes.  prefix_len 0: no prefix."""
-    _need_cache(k_cache, v_cache)
-    _need_heads(q, B * S, k_cache)
-    nh, hd = q.shape[1], q.shape[2]
-    dev = k_cache.device
-    _need(q_start, "q_start", torch.int32, 1)
-    _need_i32(q_start, "q_start", B, dev)
-    _need_i32(cache_slot, "cache_slot", B, dev)
-    _need_i32(kv_start, "kv_start", B, dev)
-    _need_batch(B, cache_slot, k_cache)
-    kp, vp, n_prefix, prefix_max = _need_prefix(k_prefix, v_prefix, prefix_len, k_cache)
-    n_slots, nkv, max_seq, _ = k_cache.shape
-    out = torch.empty((B * S, nh * hd), dtype=torch.bfloat16, device=dev)
-    lse = torch.empty((B * S, nh), dtype=torch.float32, device=dev) if return_lse else None
-    if B * S > 0:
-        _launch(dev, "qmoe_attention_prefix_prefill", _C.lib().qmoe_attention_prefix_prefill,
+    try:
+        i = k_cache.get_device()
+        n_slots, nkv, max_seq, hd = rows = k_cache.shape
+        n, nh, d = q.shape
+        if prefix_len:
+            n_prefix, pkv, prefix_max, pd = pshape = k_prefix.shape
+        good = (i >= 0 and d == hd and n == B * S and _plain(i, _BF16, q, k_cache, v_cache)
+                and _plain(i, _I32, q_start, cache_slot, kv_start) and v_cache.shape == rows
+                and q_start.shape == (B,) and (B <= n_slots if cache_slot is None else cache_slot.shape == (B,))
+                and (kv_start is None or kv_start.shape == (B,))
+                and (not prefix_len or (_plain(i, _BF16, k_prefix, v_prefix) and v_prefix.shape == pshape
+                                        and pkv == nkv and pd == hd)))
+    except (AttributeError, ValueError):
+        good = False
+    if not good:
+        _need_cache(k_cache, v_cache)
+        _need_queries(q, B, S, k_cache, q_start, cache_slot, kv_start)
+        _need_prefix(k_prefix, v_prefix, prefix_len, k_cache)
+    out = q.new_empty((n, nh * hd))
+    lse = q.new_empty((n, nh), dtype=_F32) if return_lse else None
+    if n > 0:
+        if prefix_len:
+            kp, vp = k_prefix.data_ptr(), v_prefix.data_ptr()
+        else:
+            kp = vp = None
+            n_prefix = prefix_max = 0
+        _launch(i, "qmoe_attention_prefix_prefill", _C.lib().qmoe_attention_prefix_prefill,
                 q.data_ptr(), kp, vp, n_prefix, prefix_max, prefix_slot, prefix_len, k_cache.data_ptr(),
                 v_cache.data_ptr(), q_start.data_ptr(), _ptr(cache_slot), _ptr(kv_start), B, S, nh, nkv, hd, n_slots,
                 max_seq, hd ** -0.5 if scale is None else scale, out.data_ptr(), _ptr(lse))
@@ -832,28 +893,31 @@ def attention_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor,
     (or the rows of a prompt's last S queries).  A cache slot may occur once
     per call.  ``max_len``: a bound on q_start + S (default: the cache's rows).
     Returns weights."""
-    _need_cache(k_cache, None)
-    _need_heads(q, B * S, k_cache)
-    nh, hd = q.shape[1], q.shape[2]
-    dev = k_cache.device
-    _need(lse, "lse", torch.float32, 2)
-    if tuple(lse.shape) != (B * S, nh) or lse.device != dev:
-        raise ValueError(f"lse must be ({B * S}, {nh}) on the cache's device")
-    _need(q_start, "q_start", torch.int32, 1)
-    _need_i32(q_start, "q_start", B, dev)
-    _need_i32(cache_slot, "cache_slot", B, dev)
-    _need_i32(kv_start, "kv_start", B, dev)
-    _need_batch(B, cache_slot, k_cache)
-    _need_rows(weights, "weights", torch.float32, k_cache)
-    n_slots, nkv, max_seq, _ = k_cache.shape
-    if B * S > 0:
+    try:
+        i = k_cache.get_device()
+        n_slots, nkv, max_seq, hd = rows = k_cache.shape
+        n, nh, d = q.shape
+        good = (i >= 0 and d == hd and n == B * S and _plain(i, _BF16, q, k_cache) and _plain(i, _F32, lse, weights)
+                and _plain(i, _I32, q_start, cache_slot, kv_start) and lse.shape == (n, nh)
+                and weights.shape == rows[:3] and q_start.shape == (B,)
+                and (B <= n_slots if cache_slot is None else cache_slot.shape == (B,))
+                and (kv_start is None or kv_start.shape == (B,)))
+    except (AttributeError, ValueError):
+        good = False
+    if not good:
+        _need_cache(k_cache, None)
+        _need_queries(q, B, S, k_cache, q_start, cache_slot, kv_start)
+        _need(lse, "lse", _F32, 2)
+        if tuple(lse.shape) != (B * S, q.shape[1]) or lse.device != k_cache.device:
+            raise ValueError(f"lse must be ({B * S}, {q.shape[1]}) on the cache's device")
+        _need_rows(weights, "weights", _F32, k_cache)
+    if n > 0:
         max_len = max_seq if max_len is None else max_len
-        ws = _workspace(workspace, _weights_bytes(dev.index, B, S, nh, nkv, max_len), dev)
-        _launch(dev, "qmoe_attention_weights", _C.lib().qmoe_attention_weights,
+        w, nbytes, _ws = _workspace(workspace, _weights_bytes(i, B, S, nh, nkv, max_len), q)
+        _launch(i, "qmoe_attention_weights", _C.lib().qmoe_attention_weights,
                 q.data_ptr(), lse.data_ptr(), k_cache.data_ptr(), q_start.data_ptr(), _ptr(cache_slot),
                 _ptr(kv_start), B, S, nh, nkv, hd, n_slots, max_seq, max_len,
-                hd ** -0.5 if scale is None else scale, weights.data_ptr(), 1 if accumulate else 0, ws.data_ptr(),
-                ws.shape[0])
+                hd ** -0.5 if scale is None else scale, weights.data_ptr(), 1 if accumulate else 0, w, nbytes)
     return weights
 
 
@@ -869,26 +933,34 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor
     rows below it, so the rows' order changes; kv_len (B,) becomes the new
     length and kv_start (B,) 0, both on the device.  ``max_len`` bounds
     kv_len.  A cache slot may occur once per call."""
-    _need_cache(k_cache, v_cache)
-    dev = k_cache.device
-    _need(kv_len, "kv_len", torch.int32, 1)
-    B = kv_len.shape[0]
-    _need_i32(kv_len, "kv_len", B, dev)
-    _need_i32(cache_slot, "cache_slot", B, dev)
-    _need_i32(kv_start, "kv_start", B, dev)
-    _need_batch(B, cache_slot, k_cache)
-    _need_rows(weights, "weights", torch.float32, k_cache)
-    _need_rows(tokens, "tokens", torch.int32, k_cache)
-    n_slots, nkv, max_seq, hd = k_cache.shape
+    try:
+        i = k_cache.get_device()
+        n_slots, nkv, max_seq, hd = rows = k_cache.shape
+        (B,) = kv_len.shape
+        good = (i >= 0 and _plain(i, _BF16, k_cache, v_cache) and _plain(i, _I32, tokens, kv_len, cache_slot, kv_start)
+                and _plain(i, _F32, weights) and v_cache.shape == rows and weights.shape == rows[:3]
+                and tokens.shape == rows[:3]
+                and (B <= n_slots if cache_slot is None else cache_slot.shape == (B,))
+                and (kv_start is None or kv_start.shape == (B,)))
+    except (AttributeError, ValueError):
+        good = False
+    if not good:
+        _need_cache(k_cache, v_cache)
+        _need(kv_len, "kv_len", _I32, 1)
+        dev = k_cache.device
+        _need_i32(kv_len, "kv_len", kv_len.shape[0], dev)
+        _need_i32(cache_slot, "cache_slot", kv_len.shape[0], dev)
+        _need_i32(kv_start, "kv_start", kv_len.shape[0], dev)
+        _need_batch(kv_len.shape[0], cache_slot, k_cache)
+        _need_rows(weights, "weights", _F32, k_cache)
+        _need_rows(tokens, "tokens", _I32, k_cache)
     if B == 0:
         return
     # a count, the new length, and a source and a destination per move, for every KV head
-    nbytes = B * nkv * (2 + 2 * max(0, min(keep, max_len))) * 4
-    ws = _workspace(workspace, nbytes, dev)
-    _launch(dev, "qmoe_kv_evict", _C.lib().qmoe_kv_evict,
+    w, nbytes, _ws = _workspace(workspace, B * nkv * (2 + 2 * max(0, min(keep, max_len))) * 4, k_cache)
+    _launch(i, "qmoe_kv_evict", _C.lib().qmoe_kv_evict,
             k_cache.data_ptr(), v_cache.data_ptr(), weights.data_ptr(), tokens.data_ptr(), kv_len.data_ptr(),
-            _ptr(cache_slot), _ptr(kv_start), B, nkv, hd, n_slots, max_seq, max_len, keep, recent, ws.data_ptr(),
-            ws.shape[0])
+            _ptr(cache_slot), _ptr(kv_start), B, nkv, hd, n_slots, max_seq, max_len, keep, recent, w, nbytes)
 
 
 # ----------------------------------------------------------------------------

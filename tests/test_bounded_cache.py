@@ -82,7 +82,7 @@ def p():
 
 
 def _decode(lib, p, **kw):
-    a = dict(q=p, kp=p, vp=p, n_prefix=1, prefix_max=64, slot=0, P=8, k=p, v=p, kv_len=p, B=2, nh=32, nkv=4, hd=128,
+    a = dict(q=p, kp=p, vp=p, n_prefix=1, prefix_max=600, slot=0, P=500, k=p, v=p, kv_len=p, B=2, nh=32, nkv=4, hd=128,
              n_slots=2, max_seq=64, max_len=64, scale=0.1, out=p, ws=p, bytes=1 << 30, cache_slot=None)
     a.update(kw)
     return lib.qmoe_attention_prefix_decode(
@@ -94,7 +94,7 @@ def _decode(lib, p, **kw):
 @pytest.mark.parametrize("kw,status", [
     (dict(q=None), -1), (dict(kv_len=None), -1), (dict(ws=None), -1), (dict(kp=None), -1),
     (dict(hd=64), -2), (dict(nh=30), -1), (dict(nh=128), -2), (dict(nkv=0), -1),
-    (dict(P=-1), -1), (dict(P=65), -1), (dict(slot=1), -1), (dict(slot=-1), -1),
+    (dict(P=-1), -1), (dict(P=601), -1), (dict(slot=1), -1), (dict(slot=-1), -1),
     (dict(max_len=65), -1), (dict(max_len=-1), -1), (dict(B=3), -1), (dict(B=-1), -1),
     (dict(scale=0.0), -1), (dict(scale=-1.0), -1), (dict(scale=float("inf")), -1), (dict(scale=float("nan")), -1),
     (dict(bytes=255), -4), (dict(n_slots=0), -1),
@@ -146,7 +146,9 @@ def test_evict_refusals(lib, p):
 
 def test_workspace_queries(lib):
     f = lib.qmoe_attention_prefix_decode_workspace_size
-    assert f(0, 32, 4, 100, 100, 0) == 0 and f(2, 32, 4, 0, 0, 0) > 0
+    # a short call is one kernel without parts; a long one keeps some
+    assert f(0, 32, 4, 100, 100, 0) == 0 and f(2, 32, 4, 100, 100, 0) == 0 and f(2, 32, 4, 1000, 1000, 0) > 0
+    assert f(2, 32, 4, 100, 100, 1) == 2 * 32 * 100 * 4
     # the scores of the own rows come on top: one fp32 per row and query head
     assert f(8, 32, 4, 100, 4096, 1) - f(8, 32, 4, 100, 4096, 0) == 8 * 32 * 4096 * 4
     assert lib.qmoe_kv_evict_workspace_size(2, 4, 1000, 10) == 2 * 4 * (2 + 20) * 4
