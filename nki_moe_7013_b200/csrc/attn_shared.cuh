@@ -157,6 +157,32 @@ __device__ __forceinline__ void umma_bf16_k128(uint32_t d, uint64_t adesc, uint6
   }
 }
 
+// Packed fp32 arithmetic of sm_100: two values in one register pair.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // One 16-byte chunk of a 128-byte-swizzled 64-column half tile.
 __device__ __forceinline__ uint32_t sw128_addr(uint32_t tile, int row, int chunk) {
   return tile + uint32_t(chunk >> 3) * kSdHalfBytes + uint32_t(row) * 128u + (uint32_t((chunk ^ row) & 7) << 4);

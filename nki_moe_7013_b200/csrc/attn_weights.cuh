@@ -331,6 +331,7 @@ __global__ void __launch_bounds__(kAwThreads, 1)
     const int g = warp >> 2;
     const int r = (warp & 3) * 32 + lane;
     const uint32_t s_row = tmem_base + (uint32_t((warp & 3) * 32) << 16) + g * kFaRows;
+    const f32x2 scale2 = pack2(a.scale_log2, a.scale_log2);
     float total = 0.f;
     int uses = 0;
     for (int s = 0;; ++s) {
@@ -349,7 +350,8 @@ __global__ void __launch_bounds__(kAwThreads, 1)
         if (!fa_wait_warp(&s_full[g], uses & 1, abort_flag, kDevErrWaitTimeoutEpilogue)) break;
         ++uses;
         tc_fence_after();
-        float p8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        f32x2 sum2[4] = {0, 0, 0, 0};
+        float edge[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           float v[32];
@@ -363,21 +365,26 @@ __global__ void __launch_bounds__(kAwThreads, 1)
           if (whole) {
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
-              const float4 n4 = *reinterpret_cast<const float4*>(neg + c * 32 + e);
-              const float nn[4] = {n4.x, n4.y, n4.z, n4.w};
+              const ulonglong2 n4 = *reinterpret_cast<const ulonglong2*>(neg + c * 32 + e);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) p8[(e + k) & 7] += fa_exp2(fmaf(v[e + k], a.scale_log2, nn[k]));
+              for (int k = 0; k < 4; k += 2) {
+                float x0, x1;
+                unpack2(fma2(pack2(v[e + k], v[e + k + 1]), scale2, k ? n4.y : n4.x), x0, x1);
+                sum2[((e + k) >> 1) & 3] = add2(sum2[((e + k) >> 1) & 3], pack2(fa_exp2(x0), fa_exp2(x1)));
+              }
             }
           } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
               const int col = c * 32 + e;
               const float p = fa_exp2(fmaf(v[e], a.scale_log2, neg[col]));
-              p8[e & 7] += col >= c0 && col < c1 ? p : 0.f;
+              edge[e & 3] += col >= c0 && col < c1 ? p : 0.f;
             }
           }
         }
-        total += ((p8[0] + p8[1]) + (p8[2] + p8[3])) + ((p8[4] + p8[5]) + (p8[6] + p8[7]));
+        float even, odd;
+        unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), even, odd);
+        total += whole ? even + odd : (edge[0] + edge[1]) + (edge[2] + edge[3]);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&done[sl]);
