@@ -15,10 +15,15 @@
 // shared_decode_combine_kernel joins:  M = max m,  out = sum_i 2^(m_i - M) o_i
 // / sum_i 2^(m_i - M) l_i.  The joined M and l also turn the scores of the
 // own rows, kept in fp32 by the first kernel, into attention weights.  Own
-// rows are cut by the batch's total: every part of a ragged batch holds about
-// as many rows (cutting each sequence into as many parts took 15 us instead of
-// TODO for 8 sequences of 1,400 to 4,096 rows).  Short calls run as one CTA per
-// (sequence, KV head) over prefix and own rows, without a second kernel.
+// rows are cut by the batch's total, so that every part of a ragged batch holds
+// about as many rows.  Short calls run as one CTA per (sequence, KV head) over
+// prefix and own rows, without a second kernel (5.2 us instead of 6.7 for two
+// sequences of 5 rows behind 129).
+//
+// Bound by HBM: 8 sequences of 1,400 to 4,096 rows (45 MB) stream at the copy
+// rate once the pipeline runs; 3.5 us before it (lengths, the cut, the first
+// tile's latency), 1.3 us of merging the warps and the joining kernel remain on
+// top: 21 us a call with weights, against 7 us of bytes.
 #pragma once
 
 #include "attention.cuh"
@@ -57,6 +62,7 @@ struct SharedDecodeArgs {
   int own_slots;    // parts per KV head that the own rows are cut into (at least one per sequence); 0: one per sequence
   int n_own_units, score_rows, n_out_blocks, row_blocks;
   int direct;       // one unit per (sequence, KV head), nothing to join
+  int wide;         // many parts: a block joins one row, not a warp
   int overlaps;     // the kernel before it (the tcgen05 prefix part) may still run
   float scale_log2;
 };
@@ -564,35 +570,39 @@ __device__ __forceinline__ void join_ml(const RowParts& p, int lane, float& M, f
   inv_l = L == 0.f ? 0.f : 1.f / L;
 }
 
-// Blocks [0, n_out_blocks): one warp per (sequence, head) joins the parts of
-// its output row in part order (run-to-run identical).  The blocks after
-// them: 256 own rows of one (sequence, KV head) each, one thread per row,
-// weights (+)= sum over the group's heads of exp2(s - M) / l.
+// Blocks [0, n_out_blocks): one warp per (sequence, head), or with many parts
+// one block, joins the parts of its output row in a fixed order (run-to-run
+// identical).  The blocks after them: 256 own rows of one (sequence, KV head)
+// each, one thread per row, weights (+)= sum over the group's heads of
+// exp2(s - M) / l.
 __global__ void __launch_bounds__(256) shared_decode_combine_kernel(const SharedDecodeArgs a) {
   __shared__ float sM[kSdMaxGroup], sInv[kSdMaxGroup];
+  __shared__ float4 s_acc[8][32];
   __shared__ int s_dup;
   griddep_wait();
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (int(blockIdx.x) < a.n_out_blocks) {
-    const int gw = blockIdx.x * 8 + warp;
+    const int gw = a.wide ? blockIdx.x : blockIdx.x * 8 + warp;
     if (gw >= a.B * a.nh) return;
     const int b = gw / a.nh;
     const int2 own = own_plan(a, b);
     const RowParts p = row_parts(a, own.y, own.x, b, gw % a.nh);
     float M, inv;
     join_ml(p, lane, M, inv);
+    const int first = a.wide ? warp : 0, step = a.wide ? 8 : 1;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < p.n; s0 += 8) {
+    for (int s0 = first; s0 < p.n; s0 += 8 * step) {
       float4 v[8];
       float sc[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
+        const int s = s0 + j * step;
         sc[j] = 0.f;
         v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (s0 + j < p.n) {
-          const float2 ml = p.ml(s0 + j);
-          v[j] = p.o(s0 + j, lane);
+        if (s < p.n) {
+          const float2 ml = p.ml(s);
+          v[j] = p.o(s, lane);
           if (ml.y != 0.f) sc[j] = exp2f(ml.x - M);
         }
       }
@@ -603,6 +613,19 @@ __global__ void __launch_bounds__(256) shared_decode_combine_kernel(const Shared
         acc[1] += v[j].y * sc[j];
         acc[2] += v[j].z * sc[j];
         acc[3] += v[j].w * sc[j];
+      }
+    }
+    if (a.wide) {
+      s_acc[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      __syncthreads();
+      if (warp > 0) return;
+#pragma unroll
+      for (int i = 1; i < 8; ++i) {
+        const float4 v = s_acc[i][lane];
+        acc[0] += v.x;
+        acc[1] += v.y;
+        acc[2] += v.z;
+        acc[3] += v.w;
       }
     }
     uint2 w;

@@ -18,12 +18,14 @@
 // attn_weights_join_kernel adds them in chunk order: no atomics, run-to-run
 // identical.
 //
-// Four K tiles per query tile because the query tiles come from L2: with one,
-// a 4,096-token prompt read 550 MB through it, and ran at that rate (93 us
-// without any arithmetic).  Then the exponentials bound it: 128 x 128 per tile
-// at 16 a cycle and SM are 1,024 cycles, against 512 of the products.  (A
-// quarter or a half of them as a degree-5 polynomial on the FMA pipe changed
-// nothing or cost 5 %: ten multiply-adds take as long as they save.)
+// Four K tiles per query tile: a quarter of the query tiles' traffic through L2
+// (550 MB with one, for a 4,096-token prompt: 124 us instead of 111).  Then the
+// exponentials bound it: 128 x 128 per tile at 16 a cycle and SM are 1,024
+// cycles, against 512 of the products; measured 1,250 a tile, in 111 us for a
+// 4,096-token prompt (0.62 PFLOP/s).  (A quarter or a half of the exponentials
+// as a degree-5 polynomial on the FMA pipe changed nothing or cost 5 %: ten
+// multiply-adds take as long as they save.  Three K tiles with a fourth
+// accumulator to fill ahead took 142 us.)
 #pragma once
 
 #include "attn_shared.cuh"

@@ -975,22 +975,30 @@ struct SharedDecodePlan {
   int64_t psplits, pchunk;
   int64_t own_slots, own_cap;  // parts per KV head aimed at, and at most
   bool direct;         // one CTA per (sequence, KV head) does it all
+  bool wide;           // a row has many parts to join
 };
 
-// Rows (prefix and own) up to which a sequence's keys are not cut.
-constexpr int64_t kDirectRows = 256;
+// Rows (prefix and own) up to which a sequence's keys are not cut: 512, and
+// 1,024 where the CTAs are 32 or more.  Measured, cut and uncut: 300 rows of 8
+// sequences 12.1 and 5.9 us, 500 rows of one sequence 7.9 and 7.8, 800 rows of
+// one 8.1 and 10.5, of 8 13.4 and 10.7, of 32 17.2 and 11.8.
+constexpr int64_t kDirectRows = 512;
+constexpr int64_t kDirectRowsMany = 1024, kDirectMany = 32;
 
-// Rows (sequences x heads of a group) above which the prefix part runs on the
-// tcgen05 kernel.
-constexpr int64_t kPrefixMmaRows = 64;
+// 16-row tiles x prefix rows x KV heads above which the prefix part runs on
+// the tcgen05 kernel (which reads the prefix once per 256 rows instead of 16,
+// but starts and ends slower).  Measured, warp-level and tcgen05, 4 KV heads:
+// 96 rows on 4,096 18.6 and 23.2 us, on 16,384 36.8 and 24.4; 256 rows on 1,024
+// 16.5 and 16.0, on 4,096 27.9 and 27.9, on 16,384 76.9 and 33.3.
+constexpr int64_t kPrefixMmaWork = 3 << 16;
 
 SharedDecodePlan shared_decode_plan(int64_t B, int64_t G, int64_t nkv, int64_t P, int64_t max_len) {
   SharedDecodePlan p{};
   const int64_t sms = std::max(1, num_sms(0));
   const int64_t rows = B * G;
-  p.direct = P + max_len <= kDirectRows;
+  p.direct = P + max_len <= (B * nkv >= kDirectMany ? kDirectRowsMany : kDirectRows);
   if (p.direct) return p;
-  p.tc = P > 0 && rows > kPrefixMmaRows;
+  p.tc = P > 0 && (rows + 15) / 16 * P * nkv > kPrefixMmaWork;
   if (p.tc) {
     // one CTA per SM; the split form where it leaves a CTA fewer steps
     const int64_t per_tile = qmoe::kFaRows / G, tiles = (P + qmoe::kFaRows - 1) / qmoe::kFaRows;
@@ -1023,6 +1031,12 @@ SharedDecodePlan shared_decode_plan(int64_t B, int64_t G, int64_t nkv, int64_t P
     p.own_slots = B * nkv >= 2 * sms ? 0 : std::max<int64_t>(1, 2 * sms / nkv);
     p.own_cap = p.own_slots == 0 ? B : std::min(p.own_slots + B, B * ((max_len + 127) / 128));
   }
+  // more parts (of an even batch) than two rounds of a warp's eight loads,
+  // while a block per row runs in a wave or so: 32 rows of 74 parts 26.9 us a
+  // call with a warp each and 17.6 with a block, 64 of 33 16.8 and 12.7, 256 of
+  // 10 21.4 and 21.9
+  const int64_t own_parts = p.own_slots == 0 ? 1 : std::min(p.own_slots / B + 1, (max_len + 127) / 128);
+  p.wide = p.psplits + own_parts > 16 && rows * nkv <= 4 * sms;
   return p;
 }
 
@@ -1626,7 +1640,8 @@ int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void
   QMOE_CHECK(check_shared_attention("attention_prefix_decode", head_dim, nh, nkv, n_slots, max_seq, scale));
   QMOE_CHECK(check_prefix("attention_prefix_decode", k_prefix, v_prefix, n_prefix_slots, prefix_max, prefix_slot,
                           prefix_len, nkv));
-  QMOE_REQUIRE(B >= 0 && B <= 65535 && max_len >= 0 && max_len <= max_seq && (cache_slot || B <= n_slots),
+  QMOE_REQUIRE(B >= 0 && B <= 65535 && B * nh < (int64_t(1) << 24) && max_len >= 0 && max_len <= max_seq &&
+                   (cache_slot || B <= n_slots),
                QMOE_ERR_INVALID_ARGUMENT, "attention_prefix_decode: bad sizes");
   const size_t need =
       qmoe_attention_prefix_decode_workspace_size(B, nh, nkv, prefix_len, max_len, weights != nullptr);
@@ -1701,7 +1716,8 @@ int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void
   a.own_slots = int(p.own_slots);
   a.n_own_units = int((p.direct ? B : p.own_cap) * nkv);
   a.score_rows = int(max_len);
-  a.n_out_blocks = int((B * nh + 7) / 8);
+  a.wide = p.wide ? 1 : 0;
+  a.n_out_blocks = int(p.wide ? B * nh : (B * nh + 7) / 8);
   a.row_blocks = int((max_len + qmoe::kSdCombineRows - 1) / qmoe::kSdCombineRows);
   a.direct = p.direct ? 1 : 0;
   a.overlaps = p.tc ? 1 : 0;

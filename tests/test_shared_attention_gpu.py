@@ -85,9 +85,9 @@ DECODE = [
     (3, 32, 4, 64, [0, 64, 130], None, [2, 0, 4], 0),          # a sequence with nothing but the prefix
     (3, 32, 4, 0, [0, 77, 300], [0, 77, 13], None, 0),         # no prefix: one row sees nothing, one only padding
     (5, 12, 4, 65, [33, 1, 2, 200, 63], [3, 0, 1, 199, 0], None, 0),
-    (9, 64, 4, 1000, [150] * 9, None, None, 0),                # 144 rows: the tcgen05 prefix, 16 heads per KV head
-    (40, 32, 4, 300, list(range(40)), None, None, 2),          # 320 rows: two tile pairs
-    (33, 10, 2, 131, list(range(33)), None, None, 0),          # 5 heads per KV head: tiles of 125 rows
+    (9, 64, 4, 1000, [150] * 9, None, None, 0),                # 144 rows, 16 heads per KV head
+    (40, 32, 4, 300, list(range(40)), None, None, 2),          # 320 rows
+    (33, 10, 2, 131, list(range(33)), None, None, 0),          # 5 heads per KV head
     (70, 2, 2, 127, [3] * 70, None, None, 0),
     (2, 32, 4, 5000, [4096, 700], None, None, 0),              # many parts
     (130, 8, 8, 700, [1] * 130, None, None, 0),                # one head per KV head
@@ -95,6 +95,12 @@ DECODE = [
     (2, 48, 3, 450, [63, 5], [0, 5], None, 0),
     (40, 16, 4, 0, [20 * i for i in range(40)], None, None, 0),
     (1, 16, 16, 0, [9000], [1], None, 0),
+    # enough rows on a long enough prefix for the tcgen05 kernel
+    (40, 32, 4, 3001, list(range(40)), None, None, 2),         # 320 rows: two tile pairs
+    (33, 10, 2, 12000, [40 * i for i in range(33)], [30 * i for i in range(33)], None, 0),  # tiles of 125 rows
+    (9, 64, 4, 6016, [150] * 9, None, [8, 7, 6, 5, 4, 3, 2, 1, 0], 0),
+    (12, 8, 1, 33000, [0] * 11 + [1], None, None, 0),          # 96 rows of one KV head: the keys split
+    (130, 8, 8, 4000, [1] * 130, None, None, 0),
 ]
 
 
@@ -240,6 +246,8 @@ PREFILL = [
     (2, 6, 2, 1000, 64, 333, [200, 340], [2, 0]),
     (1, 32, 4, 255, 600, 11, None, None),
     (2, 16, 1, 63, 5, 250, None, [1, 0]),
+    (2, 32, 4, 300, 700, 20, [5, 400], None),          # queries cut into chunks, padding before the first
+    (1, 10, 2, 0, 450, 0, [33], None),
 ]
 
 
@@ -461,3 +469,192 @@ def test_append_rows(cuda_dev):
             assert torch.equal(a[s, :, r], c[s, :, p])
         assert bool((tok[s, :, r] == p).all()) and not w[s, :, r].any()
     assert int((tok >= 0).sum()) == 5 * nkv and int((w == 3.0).sum()) == 2 * nkv * max_seq - 5 * nkv
+
+
+def test_evict_empty_cache(cuda_dev):
+    from nki_moe_7013_b200 import ops
+
+    k = _randn(_gen(13), 2, 2, 8, HD)
+    w, tok = torch.ones(2, 2, 8, device="cuda"), torch.ones(2, 2, 8, dtype=torch.int32, device="cuda")
+    n = _i32([0, 0])
+    ops.kv_evict(k, k.clone(), w, tok, n, 0, 4, recent=2)
+    ops.kv_evict(k[:0], k[:0], w[:0], tok[:0], _i32([]), 0, 4)
+    assert _error() == 0 and n.tolist() == [0, 0] and bool((w == 1).all()) and bool((tok == 1).all())
+
+
+@pytest.mark.parametrize("P,own", [(3001, 90), (700, 600), (100, 60)])
+def test_captured_calls_follow_their_inputs(cuda_dev, P, own):
+    """Decode with weights (the tcgen05 prefix, cut sequences, and the single
+    kernel), prefill, prompt weights and an eviction in one graph, replayed
+    with other inputs, against eager calls; two graphs, each with workspaces of
+    its own, in flight on two streams."""
+    from nki_moe_7013_b200 import ops
+
+    B, nh, nkv, S, rows = 40, 32, 4, 19, 640
+    g = _gen(P)
+    kp, vp = _randn(g, 1, nkv, P, HD), _randn(g, 1, nkv, P, HD)
+
+    def state():
+        return dict(k=_randn(g, B, nkv, rows, HD), v=_randn(g, B, nkv, rows, HD), q=_randn(g, B, nh, HD),
+                    qs=_randn(g, B * S, nh, HD), n=torch.zeros(B, dtype=torch.int32, device="cuda"),
+                    start=torch.zeros(B, dtype=torch.int32, device="cuda"),
+                    w=torch.zeros(B, nkv, rows, device="cuda"),
+                    tok=torch.arange(rows, dtype=torch.int32, device="cuda").expand(B, nkv, rows).contiguous())
+
+    def step(s):
+        out = ops.attention_prefix_decode(s["q"], kp, vp, P, s["k"], s["v"], s["n"], own, weights=s["w"])
+        pre, lse = ops.attention_prefix_prefill(s["qs"], kp, vp, P, s["k"], s["v"], s["start"], B, S, return_lse=True)
+        ops.attention_weights(s["qs"], lse, s["k"], s["start"], B, S, s["w"])
+        ops.kv_evict(s["k"], s["v"], s["w"], s["tok"], s["n"], own, 25, recent=3)
+        return out, pre, lse
+
+    def fill(s, seed):
+        r = _gen(seed)
+        for t in ("k", "v", "q", "qs"):
+            s[t].copy_(torch.randn(s[t].shape, generator=r, device="cuda"))
+        s["w"].zero_()
+        s["tok"].copy_(torch.arange(rows, device="cuda").expand(B, nkv, rows))
+        s["n"].copy_(torch.randint(1, own + 1, (B,), generator=r, device="cuda"))
+        s["start"].copy_(torch.randint(0, rows - S, (B,), generator=r, device="cuda"))
+
+    states, graphs, outs = [state(), state()], [], []
+    for s in states:
+        fill(s, 1)
+        step(s)  # outside the capture first
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(s))
+        graphs.append(graph)
+    for seed in (2, 3):
+        for i, s in enumerate(states):
+            fill(s, 10 * seed + i)
+        streams = [torch.cuda.Stream() for _ in graphs]
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for i, s in enumerate(states):
+            e = state()
+            fill(e, 10 * seed + i)
+            want = step(e)
+            torch.cuda.synchronize()
+            for got, ref in zip(outs[i], want):
+                assert torch.equal(got, ref)
+            for t in ("k", "v", "w", "tok", "n"):
+                assert torch.equal(s[t], e[t]), t
+    assert _error() == 0
+
+
+def test_offsets_past_32_bits(cuda_dev):
+    """Caches of more than 2^31 elements: the last slot's last rows."""
+    from nki_moe_7013_b200 import ops
+
+    g = _gen(14)
+    n_slots, nkv, nh, max_seq, L = 3, 8, 16, 700000, 699990
+    k = torch.zeros(n_slots, nkv, max_seq, HD, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    assert k.numel() > 2 ** 31
+    lo, S = L - 300, 40
+    k[2, :, lo:L], v[2, :, lo:L] = _randn(g, nkv, 300, HD), _randn(g, nkv, 300, HD)
+    kk, vv = k[2, :, lo:L].clone(), v[2, :, lo:L].clone()
+    q, qs = _randn(g, 1, nh, HD), _randn(g, S, nh, HD)
+    w = torch.zeros(n_slots, nkv, max_seq, device="cuda")
+    tok = torch.arange(max_seq, dtype=torch.int32, device="cuda").expand(n_slots, nkv, max_seq).contiguous()
+    slot, start = _i32([2]), _i32([lo])
+    out = ops.attention_decode_weights(q, k, v, _i32([L]), L, w, cache_slot=slot, kv_start=start)
+    wide = ops.attention_prefix_decode(q, k, v, L, k, v, _i32([0]), 0, prefix_slot=2)  # a prefix past 2^31
+    pre, lse = ops.attention_prefix_prefill(qs, None, None, 0, k, v, _i32([L - S]), 1, S, cache_slot=slot,
+                                            kv_start=start, return_lse=True)
+    w2 = torch.zeros_like(w)
+    ops.attention_weights(qs, lse, k, _i32([L - S]), 1, S, w2, cache_slot=slot, kv_start=start, max_len=L)
+    assert _error() == 0
+    for gr in range(nkv):
+        h = slice(gr * 2, gr * 2 + 2)
+        r = Ref(q[0, h], kk[gr], vv[gr])
+        _check_out(out.view(nh, HD)[h], r.out, r.mag, r.D)
+        _check_weights(w[2, gr, lo:L], r.p.sum(dim=0), torch.zeros(300, dtype=torch.float64, device="cuda"), r.D)
+        # the rows before `lo` hold zeros: scores of 0 and no value
+        s = torch.cat([torch.exp(q[0, h].double() @ kk[gr].double().T * C), torch.full((2, 1), float(lo), device="cuda",
+                                                                                       dtype=torch.float64)], dim=1)
+        p = s[:, :300] / s.sum(dim=1, keepdim=True)
+        _check_out(wide.view(nh, HD)[h], p @ vv[gr].double(), p @ vv[gr].double().abs(), r.D)
+    hide = torch.arange(lo, L, device="cuda")[None] > torch.arange(L - S, L, device="cuda")[:, None]
+    for h in range(nh):
+        r = Ref(qs[:, h], kk[h // 2], vv[h // 2], hide)
+        _check_out(pre.view(S, nh, HD)[:, h], r.out, r.mag, r.D)
+    assert abs(float(w2.double().sum()) - S * nh) <= S * nh * 2.0 ** -12
+    assert not w2[:2].any() and not w2[2, :, :lo].any() and not w2[2, :, L:].any()
+    n = _i32([L])
+    ops.kv_evict(k, v, w, tok, n, L, 100, recent=10, cache_slot=slot, kv_start=start)
+    assert _error() == 0 and n.tolist() == [100] and start.tolist() == [0]
+    assert bool((tok[2, :, :100] >= lo).all()) and bool((tok[2, :, 100:L] == -1).all())
+    for gr in range(nkv):
+        rows = tok[2, gr, :100].long() - lo
+        assert torch.equal(k[2, gr, :100], kk[gr, rows]) and torch.equal(v[2, gr, :100], vv[gr, rows])
+        assert set(range(290, 300)) <= set(rows.tolist()) and len(set(rows.tolist())) == 100
+
+
+def test_wrappers_refuse_what_does_not_fit(cuda_dev):
+    """Wrong types, shapes, layouts: refused with a name, before a launch."""
+    from nki_moe_7013_b200 import _C, ops
+
+    B, nh, nkv, L = 2, 8, 2, 16
+    bf = dict(dtype=torch.bfloat16, device="cuda")
+    k, v, q = torch.zeros(B, nkv, L, HD, **bf), torch.zeros(B, nkv, L, HD, **bf), torch.zeros(B, nh, HD, **bf)
+    n, w = _i32([3, 4]), torch.zeros(B, nkv, L, device="cuda")
+    lse, tok = torch.zeros(B, nh, device="cuda"), torch.zeros(B, nkv, L, dtype=torch.int32, device="cuda")
+
+    def decode(**kw):
+        a = dict(q=q, k_prefix=k, v_prefix=v, prefix_len=4, k_cache=k, v_cache=v, kv_len=n, max_len=L)
+        a.update(kw)
+        return ops.attention_prefix_decode(**a)
+
+    def prefill(**kw):
+        a = dict(q=q, k_prefix=k, v_prefix=v, prefix_len=4, k_cache=k, v_cache=v, q_start=n, B=B, S=1)
+        a.update(kw)
+        return ops.attention_prefix_prefill(**a)
+
+    def weights(**kw):
+        a = dict(q=q, lse=lse, k_cache=k, q_start=n, B=B, S=1, weights=w)
+        a.update(kw)
+        return ops.attention_weights(**a)
+
+    def evict(**kw):
+        a = dict(k_cache=k, v_cache=v, weights=w, tokens=tok, kv_len=n.clone(), max_len=L, keep=3)
+        a.update(kw)
+        return ops.kv_evict(**a)
+
+    for call in (decode, prefill, weights, evict):
+        call()
+    half = torch.zeros(B, nkv, L, HD, dtype=torch.float16, device="cuda")
+    strided = torch.zeros(B, nkv, HD, L, **bf).transpose(2, 3)
+    for call, kw, err, name in (
+            (decode, dict(q=q.float()), TypeError, "q must"), (decode, dict(q=None), TypeError, "q must"),
+            (decode, dict(k_cache=half), TypeError, "k_cache"), (decode, dict(v_cache=strided), ValueError, "v_cache"),
+            (decode, dict(q=q[:1].contiguous()), ValueError, "q must"), (decode, dict(kv_len=n.long()), TypeError, "kv_len"),
+            (decode, dict(kv_len=n.view(1, 2)), ValueError, "kv_len"), (decode, dict(kv_start=n[:1]), ValueError, "kv_start"),
+            (decode, dict(k_prefix=None), ValueError, "prefix"), (decode, dict(v_prefix=k[:1].contiguous()), ValueError, "prefix"),
+            (decode, dict(k_prefix=k[:, :1].contiguous(), v_prefix=v[:, :1].contiguous()), ValueError, "prefix"),
+            (decode, dict(weights=w[:1].contiguous()), ValueError, "weights"), (decode, dict(weights=w.half()), TypeError, "weights"),
+            (decode, dict(workspace=torch.zeros(4, device="cuda")), TypeError, "workspace"),
+            (decode, dict(q=torch.zeros(3, nh, HD, **bf), kv_len=_i32([1, 1, 1])), ValueError, "cache_slot"),
+            (decode, dict(prefix_len=17), _C.QmoeError, "prefix"), (decode, dict(prefix_slot=2), _C.QmoeError, "prefix"),
+            (decode, dict(max_len=17), _C.QmoeError, "sizes"), (decode, dict(scale=0.0), _C.QmoeError, "scale"),
+            (decode, dict(q=torch.zeros(B, 7, HD, **bf)), _C.QmoeError, "heads"),
+            (prefill, dict(q_start=n.float()), TypeError, "q_start"), (prefill, dict(S=2), ValueError, "q must"),
+            (prefill, dict(cache_slot=n[:1]), ValueError, "cache_slot"), (prefill, dict(prefix_len=-1), _C.QmoeError, "prefix"),
+            (weights, dict(lse=lse.double()), TypeError, "lse"), (weights, dict(lse=lse[:1].contiguous()), ValueError, "lse"),
+            (weights, dict(weights=tok), TypeError, "weights"), (weights, dict(max_len=0), _C.QmoeError, "sizes"),
+            (evict, dict(tokens=tok.long()), TypeError, "tokens"), (evict, dict(v_cache=k[:1].contiguous()), ValueError, "cache"),
+            (evict, dict(keep=-1), _C.QmoeError, "recent"), (evict, dict(recent=4), _C.QmoeError, "recent"),
+            (evict, dict(kv_len=n.tolist()), TypeError, "kv_len")):
+        with pytest.raises(err, match=name):
+            call(**kw)
+    with pytest.raises(TypeError, match="weights"):
+        ops.attention_decode_weights(q, k, v, n, L, None)
+    with pytest.raises(ValueError, match="together"):
+        ops.qk_norm_rope(torch.zeros(1, 12 * HD, **bf), n[:1].contiguous(), torch.ones(HD, device="cuda"),
+                         torch.ones(HD, device="cuda"), torch.ones(64, device="cuda"), nh, nkv, 1e-6, k, v,
+                         row_tokens=tok)
+    assert _error() == 0
