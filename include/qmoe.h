@@ -461,8 +461,11 @@ QMOE_API int qmoe_attention_decode(const void* q, const void* k_cache, const voi
  *   prefix_len 0: none (the pointers may be NULL).  It may be a slot of
  *   k_cache / v_cache.
  * Own rows: kv_start[b] .. of slot cache_slot[b] (NULL: slot b), as in
- *   qmoe_attention_prefill / _decode.  Rows outside the visible ranges, and
- *   what they hold (NaN and infinities included), reach no output.
+ *   qmoe_attention_prefill / _decode.  Rows that no query of the call sees,
+ *   and what they hold (NaN and infinities included), reach no output.  In a
+ *   prefill a value row that is not finite makes NaN of the dims that are not
+ *   for every query of the row tiles that reach it, the earlier queries of
+ *   such a tile, which do not see the row, included (0 x inf).
  * weights (n_slots, nkv, max_seq) fp32: weights[slot, g, j] becomes (with
  *   accumulate: += ) the sum over the KV head's query heads, and over the
  *   queries, of the attention probability of own row j; without accumulate

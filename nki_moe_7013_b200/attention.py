@@ -113,6 +113,25 @@ class KVCache:
         self._clear_positions(self.n_slots)
         return self
 
+    def _follow(self, prefix_len: int, pads: Optional[List[int]], B: int) -> None:
+        """The host's side of a call that appends to slots 0 .. B-1 behind
+        ``prefix_len`` shared rows: refuses what the rows already there
+        contradict, and records paddings (``pads``; None: as they are) and the
+        distance of a new row's position from the row."""
+        for b in range(B):
+            fresh = self.lengths[b] == 0 and self.dropped[b] == 0
+            if not fresh and self.prefix_len[b] != prefix_len:
+                raise ValueError("the cache was filled behind another prefix (or none)")
+            if prefix_len and pads is not None and pads[b] != self.pad[b] and pads[b] < self.lengths[b]:
+                raise ValueError("attention_mask: behind a prefix the paddings come with a sequence's first tokens")
+        for b in range(B):
+            if pads is not None:
+                self.pad[b] = self.lead[b] = pads[b]
+            if self.dropped[b] == 0 and self.lengths[b] <= self.pad[b]:  # no token yet
+                # behind a prefix the distance to it counts, so paddings are left out of the positions
+                self.prefix_len[b] = prefix_len
+                self.offset[b] = prefix_len - self.pad[b] if prefix_len else 0
+
     def as_prefix(self, slot: int = 0) -> "SharedPrefix":
         """The rows of one slot as a prefix for other sequences (no copy: the
         slot must not change while the prefix is in use)."""
@@ -282,21 +301,11 @@ class Qwen3MoeAttention(nn.Module):
             raise ValueError("KV cache is full")
         x2d = hidden_states.reshape(B * S, H).to(torch.bfloat16).contiguous()
         P = prefix.length if prefix is not None else 0
-        fresh = [l0 == 0 and n == 0 for l0, n in zip(L0, cache.dropped)]
         if P and prefix.k is cache.k and prefix.slot < B:
             raise ValueError("the prefix's slot is one of the batch's own")
-        if any(not f and p != P for f, p in zip(fresh, cache.prefix_len)):
-            raise ValueError("the cache was filled behind another prefix (or none)")
         if attention_mask is not None and any(cache.dropped[:B]):
             raise ValueError("attention_mask: the cache evicted rows (its paddings among them); pass no mask")
-        pads = left_padding(attention_mask, B, S, L0)
-        for b in range(B):
-            if pads is not None:
-                cache.pad[b] = cache.lead[b] = pads[b]
-            if fresh[b]:
-                # behind a prefix the distance to it counts, so paddings are left out of the positions
-                cache.prefix_len[b] = P
-                cache.offset[b] = P - cache.pad[b] if P else 0
+        cache._follow(P, left_padding(attention_mask, B, S, L0), B)
         pad_now = cache.pad[:B]
         rows = (torch.tensor(L0, dtype=torch.int32).unsqueeze(1) + torch.arange(S, dtype=torch.int32))
         pos = rows + torch.tensor(cache.offset[:B], dtype=torch.int32).unsqueeze(1)

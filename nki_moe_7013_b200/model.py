@@ -145,6 +145,8 @@ class Qwen3MoeModel:
         """Run one prompt (P,) or (1, P) and return its rows in every layer as
         a prefix that batches can share."""
         ids = input_ids.reshape(1, -1)
+        if ids.shape[1] == 0 or input_ids.shape[-1] != ids.shape[1]:
+            raise ValueError(f"prefill_prefix takes one prompt of at least one token (got {tuple(input_ids.shape)})")
         caches = self.new_caches(1, ids.shape[1])
         self.hidden_states(ids, caches)
         return [c.as_prefix() for c in caches]

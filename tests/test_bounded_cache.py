@@ -50,6 +50,36 @@ def test_cache_refusals():
         c.as_prefix(1)
 
 
+def test_paddings_behind_a_prefix():
+    c = _cache()
+    c._follow(5, [0, 2, 4], 3)
+    assert c.offset == [5, 3, 1] and c.prefix_len == [5, 5, 5] and c.lead == [0, 2, 4]
+    c.lengths = [4, 4, 4]  # the third holds paddings alone
+    for pads in ([1, 2, 4], [0, 0, 4], [0, 2, 3]):
+        with pytest.raises(ValueError, match="first tokens"):
+            c._follow(5, pads, 3)
+    with pytest.raises(ValueError, match="another prefix"):
+        c._follow(6, None, 3)
+    assert c.offset == [5, 3, 1] and c.pad == [0, 2, 4]
+    c._follow(5, [0, 2, 6], 3)  # its first token comes at row 6, at position 5
+    assert c.offset == [5, 3, -1] and c.pad == [0, 2, 6]
+    c.lengths = [8, 8, 8]
+    c._follow(5, None, 3)
+    assert c.offset == [5, 3, -1]
+    # without a prefix a row's position is the row
+    d = _cache()
+    d._follow(0, [0, 2, 4], 3)
+    assert d.offset == [0, 0, 0] and d.pad == [0, 2, 4]
+
+
+def test_a_prefix_is_one_prompt():
+    from nki_moe_7013_b200.model import Qwen3MoeModel
+
+    for ids in (torch.zeros(2, 3, dtype=torch.int64), torch.zeros(0, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="one prompt"):
+            Qwen3MoeModel.prefill_prefix(object.__new__(Qwen3MoeModel), ids)
+
+
 def test_wrappers_refuse_cpu_tensors():
     k = torch.zeros(2, 2, 16, 128, dtype=torch.bfloat16)
     q = torch.zeros(2, 8, 128, dtype=torch.bfloat16)

@@ -44,6 +44,23 @@ def test_attention_behind_a_prefix_equals_the_whole_sequence(cuda_dev, P):
     assert _C.device_error() == 0
 
 
+def test_a_first_chunk_of_paddings_behind_a_prefix(cuda_dev):
+    """Prompts in two chunks, the second sequence's first token in the second
+    one, against each sequence run whole."""
+    attn, H = _attn(cuda_dev, seed=9)
+    P, B, S, cut, pads = 33, 2, 24, 10, [3, 14]
+    xp = activations(11, P, H, cuda_dev).view(1, P, H)
+    x = activations(12, B * S, H, cuda_dev).view(B, S, H)
+    prefix = attn(xp)[1].as_prefix()
+    cache = attn.new_cache(B, S)
+    mask = (torch.arange(S)[None] >= torch.tensor(pads)[:, None]).int()
+    got = torch.cat([attn(x[:, :cut], None, cache, attention_mask=mask[:, :cut], prefix=prefix)[0],
+                     attn(x[:, cut:], None, cache, attention_mask=mask, prefix=prefix)[0]], dim=1)
+    for b in range(B):
+        whole, _ = attn(torch.cat([xp, x[b:b + 1, pads[b]:]], dim=1))
+        assert max_rel_err(to_f32_np(got[b, pads[b]:]), to_f32_np(whole[0, P:])) <= MAX_REL
+
+
 def test_prefix_refusals(cuda_dev):
     attn, H = _attn(cuda_dev)
     x = activations(3, 2 * 6, H, cuda_dev).view(2, 6, H)
