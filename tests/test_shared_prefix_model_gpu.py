@@ -219,6 +219,40 @@ def test_bounded_session_replay_matches_eager_steps(cuda_dev, with_prefix):
         assert bool((a.tokens[:, :, used:] == -1).all()) and not a.weights[:, :, used:].any()
 
 
+@pytest.mark.parametrize("keep", [None, 24])
+def test_session_after_its_prompts(cuda_dev, keep):
+    """Prompts behind a prefix prefilled into a session's caches, then steps,
+    against the module path over the same tokens (and, with ``keep``, the same
+    evictions)."""
+    from nki_moe_7013_b200 import _C
+    from nki_moe_7013_b200.model import DecodeSession
+
+    model = _small_model(cuda_dev, seed=10)
+    prefix = model.prefill_prefix(torch.randint(0, 2048, (70,), device=cuda_dev))
+    B, S = 2, 30
+    ids = torch.randint(0, 2048, (B, S), device=cuda_dev)
+    sess = DecodeSession(model, B, context=S, max_new=3, prefix=prefix, keep=keep, recent=8 if keep else 0,
+                         fill_random=False, split_k=False)
+    logits, _ = model.forward(ids, sess.caches, last_only=True, prefix=prefix)
+    caches = model.new_caches(B, S + 3, track=keep is not None)
+    ref, _ = model.forward(ids, caches, last_only=True, prefix=prefix)
+    assert max_rel_err(to_f32_np(logits), to_f32_np(ref)) <= MAX_REL
+    sess.tokens.copy_(logits[:, -1].argmax(-1))
+    for step in range(3 if keep is None else 8):
+        if keep is not None and caches[0].lengths[0] == S + 3:
+            for c, s in zip(caches, sess.caches):  # near ties may fall apart: the totals that decide are shared
+                c.weights.copy_(s.weights)
+                c.evict(keep, recent=8)
+        tokens = sess.tokens.clone()
+        ref, _ = model.forward(tokens.reshape(B, 1), caches, prefix=prefix)
+        sess.step()
+        assert max_rel_err(to_f32_np(sess.logits), to_f32_np(ref.reshape(B, -1))) <= MAX_REL, step
+    for c, s in zip(caches, sess.caches):
+        if keep is not None:
+            assert torch.equal(c.tokens, s.tokens)
+    assert _C.device_error() == 0
+
+
 def test_session_refusals(cuda_dev):
     from nki_moe_7013_b200.model import DecodeSession
 
