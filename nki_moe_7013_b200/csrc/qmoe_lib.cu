@@ -986,11 +986,13 @@ constexpr int64_t kDirectRows = 512;
 constexpr int64_t kDirectRowsMany = 1024, kDirectMany = 32;
 
 // 16-row tiles x prefix rows x KV heads above which the prefix part runs on
-// the tcgen05 kernel (which reads the prefix once per 256 rows instead of 16,
-// but starts and ends slower).  Measured, warp-level and tcgen05, 4 KV heads:
-// 96 rows on 4,096 18.6 and 23.2 us, on 16,384 36.8 and 24.4; 256 rows on 1,024
-// 16.5 and 16.0, on 4,096 27.9 and 27.9, on 16,384 76.9 and 33.3.
-constexpr int64_t kPrefixMmaWork = 3 << 16;
+// the tcgen05 kernel (which reads the prefix once per 128 rows instead of 16,
+// beside the own rows, but starts and ends slower); a single tile reads it once
+// anyway.  Measured with 4 KV heads, warp-level and tcgen05: 64 rows on 1,024
+// (16,384) 12.4 and 15.3 us, on 2,048 14.1 and 13.4; 256 rows on 512 (32,768)
+// 19.7 and 18.5, on 2,048 24.8 and 20.7; 1,024 rows on 130 45.5 and 38.5; one
+// tile on 16,384 (65,536) 15.5 and 18.0.
+constexpr int64_t kPrefixMmaWork = 3 << 13;
 
 SharedDecodePlan shared_decode_plan(int64_t B, int64_t G, int64_t nkv, int64_t P, int64_t max_len) {
   SharedDecodePlan p{};
@@ -998,24 +1000,39 @@ SharedDecodePlan shared_decode_plan(int64_t B, int64_t G, int64_t nkv, int64_t P
   const int64_t rows = B * G;
   p.direct = P + max_len <= (B * nkv >= kDirectMany ? kDirectRowsMany : kDirectRows);
   if (p.direct) return p;
-  p.tc = P > 0 && (rows + 15) / 16 * P * nkv > kPrefixMmaWork;
+  p.tc = rows > 16 && (rows + 15) / 16 * P * nkv > kPrefixMmaWork;
   if (p.tc) {
-    // one CTA per SM; the split form where it leaves a CTA fewer steps
+    // The own rows' kernel fills the SMs that the prefix part leaves free, so
+    // the more parts, the sooner the prefix is done and the longer the own rows
+    // run on after it.  Taken is the form and number of parts of the least
+    // estimate: steps of 1.9 us, and one to join a split tile's halves; own rows
+    // (max_len / 2 of them, their lengths being on the device) at 30 GB/s per
+    // free SM beside them and at 6 TB/s after them; 0.75 us per part of 4,096
+    // rows written and joined; up to 6 us where the last SMs are taken too.
+    // Fitted to 90 cuts of 11 shapes, of which it picks the best or one within
+    // 2 % in 10.  Measured, 128 sequences on 16,384 rows, up to 640 own rows:
+    // split, 2 parts 76.6 us, 3 57.6, 4 64.2; unsplit, 5 67.6, 6 61.1, 9 71.1.
     const int64_t per_tile = qmoe::kFaRows / G, tiles = (P + qmoe::kFaRows - 1) / qmoe::kFaRows;
     const int64_t row_tiles = (B + per_tile - 1) / per_tile;
-    double best = 0;
+    const double own_mb = double(B * nkv) * double(max_len) * 0.5 * 512e-6, part_us = double(rows * nkv) * (0.75 / 4096);
+    double best = -1;
     for (int split = 0; split < 2; ++split) {
-      const int64_t blocks = split ? row_tiles : (row_tiles + 1) / 2;
-      const int64_t want = std::max<int64_t>(1, std::min(tiles, sms / (blocks * nkv)));
-      const int64_t per_part = (tiles + want - 1) / want, parts = (tiles + per_part - 1) / per_part;
-      const double waves = double((blocks * nkv * parts + sms - 1) / sms);
-      const double cost = waves * (split ? double((per_part + 1) / 2 + 1) : double(per_part));
-      if (split && cost >= best) break;
-      best = cost;
-      p.split = split != 0;
-      p.row_tiles = blocks;
-      p.pchunk = per_part * qmoe::kFaRows;
-      p.psplits = parts;
+      const int64_t columns = (split ? row_tiles : (row_tiles + 1) / 2) * nkv;
+      const int64_t most = std::max<int64_t>(1, std::min(tiles, sms / columns));
+      for (int64_t want = 1; want <= most; ++want) {
+        const int64_t per_part = (tiles + want - 1) / want, parts = (tiles + per_part - 1) / per_part;
+        const int64_t ctas = columns * parts;
+        const double t = 1.9 * double((ctas + sms - 1) / sms) * double(split ? (per_part + 1) / 2 + 1 : per_part);
+        const double beside = double(std::max<int64_t>(0, sms - ctas)) * t * 0.03;
+        const double full = std::max(0.0, std::min(1.0, double(ctas) / double(sms)) - 0.5) * 12;
+        const double cost = t + std::max(0.0, own_mb - beside) / 6 + part_us * double(parts) + full;
+        if (best >= 0 && cost >= best) continue;
+        best = cost;
+        p.split = split != 0;
+        p.row_tiles = columns / nkv;
+        p.pchunk = per_part * qmoe::kFaRows;
+        p.psplits = parts;
+      }
     }
   } else if (P > 0) {
     // two CTAs per SM, parts of at least 128 keys
@@ -1038,6 +1055,12 @@ SharedDecodePlan shared_decode_plan(int64_t B, int64_t G, int64_t nkv, int64_t P
   const int64_t own_parts = p.own_slots == 0 ? 1 : std::min(p.own_slots / B + 1, (max_len + 127) / 128);
   p.wide = p.psplits + own_parts > 16 && rows * nkv <= 4 * sms;
   return p;
+}
+
+size_t shared_decode_bytes(const SharedDecodePlan& p, int64_t B, int64_t nh, int64_t max_len, bool with_weights) {
+  const size_t rows = size_t(B * nh * p.psplits + p.own_cap * nh);
+  const size_t scores = with_weights ? size_t(B * nh) * size_t(max_len) * sizeof(float) : 0;
+  return p.direct ? scores : rows * (qmoe::kAttnD + 2) * sizeof(float) + size_t(B) * sizeof(int2) + scores;
 }
 
 // How the queries that score a cache are cut: blocks of 512 rows, each
@@ -1623,10 +1646,8 @@ int qmoe_attention_decode(const void* q, const void* k_cache, const void* v_cach
 size_t qmoe_attention_prefix_decode_workspace_size(int64_t B, int64_t nh, int64_t nkv, int64_t prefix_len,
                                                    int64_t max_len, int with_weights) {
   if (B <= 0 || nkv <= 0 || nh <= 0 || nh % nkv != 0 || prefix_len < 0 || max_len < 0) return 0;
-  const SharedDecodePlan p = shared_decode_plan(B, nh / nkv, nkv, prefix_len, max_len);
-  const size_t rows = size_t(B * nh * p.psplits + p.own_cap * nh);
-  const size_t scores = with_weights ? size_t(B * nh) * size_t(max_len) * sizeof(float) : 0;
-  return p.direct ? scores : rows * (qmoe::kAttnD + 2) * sizeof(float) + size_t(B) * sizeof(int2) + scores;
+  return shared_decode_bytes(shared_decode_plan(B, nh / nkv, nkv, prefix_len, max_len), B, nh, max_len,
+                             with_weights != 0);
 }
 
 int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void* v_prefix, int64_t n_prefix_slots,
@@ -1643,8 +1664,9 @@ int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void
   QMOE_REQUIRE(B >= 0 && B <= 65535 && B * nh < (int64_t(1) << 24) && max_len >= 0 && max_len <= max_seq &&
                    (cache_slot || B <= n_slots),
                QMOE_ERR_INVALID_ARGUMENT, "attention_prefix_decode: bad sizes");
-  const size_t need =
-      qmoe_attention_prefix_decode_workspace_size(B, nh, nkv, prefix_len, max_len, weights != nullptr);
+  const int64_t G = nh / nkv;
+  const SharedDecodePlan p = B > 0 ? shared_decode_plan(B, G, nkv, prefix_len, max_len) : SharedDecodePlan{};
+  const size_t need = B > 0 ? shared_decode_bytes(p, B, nh, max_len, weights != nullptr) : 0;
   QMOE_REQUIRE(workspace || need == 0, QMOE_ERR_INVALID_ARGUMENT, "attention_prefix_decode: null workspace");
   QMOE_REQUIRE(workspace_bytes >= need, QMOE_ERR_WORKSPACE_TOO_SMALL,
                "attention_prefix_decode: workspace too small");
@@ -1654,8 +1676,6 @@ int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void
   DeviceInfo* d = nullptr;
   QMOE_CHECK(device_info(&d));
   if (B == 0) return QMOE_OK;
-  const int64_t G = nh / nkv;
-  const SharedDecodePlan p = shared_decode_plan(B, G, nkv, prefix_len, max_len);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   qmoe::SharedDecodeArgs a{};
   a.pre_o = static_cast<float*>(workspace);
