@@ -27,6 +27,7 @@ constexpr int kEvWarps = kEvThreads / 32;
 constexpr int kEvMaxCached = 32768;  // order keys a CTA holds in shared memory (128 KB); rows past it are re-read from L2
 constexpr int kEvMaxCluster = 8;
 constexpr int kEvMoveRows = 32;      // rows per CTA of the move kernel
+constexpr int kEvHeld = 4;           // rows of a thread whose weight and token are read once, into registers
 
 struct EvictArgs {
   float* weights;    // (n_slots, nkv, max_seq)
@@ -82,9 +83,9 @@ __device__ __forceinline__ int ld_cluster(const int* p, int rank) {
 
 __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const EvictArgs a) {
   extern __shared__ uint32_t ev_keys[];  // of this CTA's first a.cached rows
-  __shared__ int hist[2][256];           // read by the whole cluster
+  __shared__ alignas(16) int hist[2][256];  // read by the whole cluster
   __shared__ int s_newest, s_eq, s_holes, s_moves;
-  __shared__ int hsum[256];
+  __shared__ alignas(16) int hsum[256];
   __shared__ int wsum[kEvWarps], wsum2[kEvWarps];
   __shared__ int s_pick, s_rest, s_count;
   griddep_wait();
@@ -118,11 +119,24 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const Evict
   const int run = ((s1 - s0 + warps - 1) / warps + 31) / 32 * 32;
   const int r_begin = min(s1, s0 + warp * run), r_end = min(s1, r_begin + run);
 
-  // the newest token
+  // the newest token; the first rows' weights are read along with their tokens
+  float w_held[kEvHeld];
+  int t_held[kEvHeld];
   int newest = INT32_MIN;
+  if (!all && n > 0) {
+#pragma unroll
+    for (int i = 0; i < kEvHeld; ++i) {
+      const int r = s0 + i * threads + tid;
+      const bool live = r >= lo && r < s1;
+      w_held[i] = live ? w[r] : 0.f;
+      t_held[i] = live && a.recent > 0 ? tok[r] : INT32_MIN;
+    }
+  }
   if (a.recent > 0 && !all) {
-#pragma unroll 4
-    for (int r = max(lo, s0) + tid; r < s1; r += threads) newest = max(newest, tok[r]);
+#pragma unroll
+    for (int i = 0; i < kEvHeld; ++i) newest = max(newest, t_held[i]);
+    for (int r = s0 + kEvHeld * threads + tid; r < s1; r += threads)
+      if (r >= lo) newest = max(newest, tok[r]);
     newest = __reduce_max_sync(0xFFFFFFFFu, newest);
     if (lane == 0) wsum[warp] = newest;
     __syncthreads();
@@ -146,17 +160,21 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const Evict
   if (!all && n > 0) {
     for (int i = tid; i < 512; i += threads) hist[i >> 8][i & 255] = 0;
     __syncthreads();
-#pragma unroll 4
-    for (int r0 = s0; r0 < s1; r0 += threads) {
-      const int r = r0 + tid;
-      const bool live = r >= lo && r < s1;
-      uint32_t k = 0;
-      if (live) {
-        k = fresh_key(r);
-        if (r - s0 < a.cached) ev_keys[r - s0] = k;
-      }
+    auto count = [&](int r, bool live, uint32_t k) {
+      if (live && r - s0 < a.cached) ev_keys[r - s0] = k;
       const uint32_t same = __match_any_sync(0xFFFFFFFFu, live ? k >> 24 : 256u);
       if (live && lane == __ffs(same) - 1) atomicAdd(&hist[0][k >> 24], __popc(same));
+    };
+#pragma unroll
+    for (int i = 0; i < kEvHeld; ++i) {
+      const int r = s0 + i * threads + tid;
+      if (s0 + i * threads < s1)
+        count(r, r >= lo && r < s1, evict_key(w_held[i], a.recent > 0 && (long long)t_held[i] > old_most));
+    }
+    for (int r0 = s0 + kEvHeld * threads; r0 < s1; r0 += threads) {
+      const int r = r0 + tid;
+      const bool live = r >= lo && r < s1;
+      count(r, live, live ? fresh_key(r) : 0u);
     }
     uint32_t mask = 0xFF000000u;
     int want = n;
@@ -177,12 +195,12 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const Evict
       }
       if (warp == 0) {
         // lane i holds digits 255-8i .. 248-8i, largest first
-        int c[8], sum = 0;
+        const int4 lo4 = *reinterpret_cast<const int4*>(h + 248 - lane * 8);
+        const int4 hi4 = *reinterpret_cast<const int4*>(h + 252 - lane * 8);
+        const int c[8] = {hi4.w, hi4.z, hi4.y, hi4.x, lo4.w, lo4.z, lo4.y, lo4.x};
+        int sum = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          c[e] = h[255 - lane * 8 - e];
-          sum += c[e];
-        }
+        for (int e = 0; e < 8; ++e) sum += c[e];
         int incl = sum;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -243,27 +261,49 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const Evict
     }
     __syncthreads();
   }
-  // two passes: count the free rows below n and the kept rows beyond it, then list them
-  int holes_before = 0, moves_before = 0, n_moves = 0;
+  // two passes: count the free rows below n and the kept rows beyond it, then
+  // list them; lane i keeps the i-th 32 rows' masks for the second pass
+  int holes_before = 0, moves_before = 0, n_moves = 0, e_later = 0;
+  uint32_t held_holes = 0, held_moves = 0;
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
-    int e = eq_before, holes = holes_before, moves = moves_before;
-    for (int r0 = r_begin; r0 < r_end; r0 += 32) {
+    int e = pass == 0 ? eq_before : e_later, holes = holes_before, moves = moves_before;
+    for (int r0 = r_begin, it = 0; r0 < r_end; r0 += 32, ++it) {
       const int r = r0 + lane;
-      const bool live = r < r_end && r >= lo;
-      bool kept = live && all;
-      if (!all && n > 0) {
-        const uint32_t k = live ? key_at(r) : 0u;
-        const bool is_eq = live && k == T;
-        const uint32_t eqs = __ballot_sync(0xFFFFFFFFu, is_eq);
-        kept = live && (k > T || (is_eq && (take_eq == INT32_MAX || e + __popc(eqs & before) < take_eq)));
-        e += __popc(eqs);
+      uint32_t hs, ms;
+      if (pass == 1 && it < 32) {
+        hs = __shfl_sync(0xFFFFFFFFu, held_holes, it);
+        ms = __shfl_sync(0xFFFFFFFFu, held_moves, it);
+      } else {
+        const bool live = r < r_end && r >= lo;
+        bool kept = live && all;
+        if (!all && n > 0) {
+          const uint32_t k = live ? key_at(r) : 0u;
+          const bool is_eq = live && k == T;
+          kept = live && (k > T || is_eq);
+          if (take_eq != INT32_MAX) {
+            const uint32_t eqs = __ballot_sync(0xFFFFFFFFu, is_eq);
+            kept = kept && (!is_eq || e + __popc(eqs & before) < take_eq);
+            e += __popc(eqs);
+          }
+        }
+        hs = __ballot_sync(0xFFFFFFFFu, r < r_end && r < n && !kept);
+        ms = __ballot_sync(0xFFFFFFFFu, kept && r >= n);
+        if (lane == it) {
+          held_holes = hs;
+          held_moves = ms;
+        }
+        if (it == 31 && pass == 0) e_later = e;
       }
-      const bool hole = r < r_end && r < n && !kept, move = kept && r >= n;
-      const uint32_t hs = __ballot_sync(0xFFFFFFFFu, hole), ms = __ballot_sync(0xFFFFFFFFu, move);
+      const bool hole = hs >> lane & 1, move = ms >> lane & 1;
       if (pass == 1) {
         if (hole) dst[holes + __popc(hs & before)] = r;
-        if (move) src[moves + __popc(ms & before)] = r;
+        if (move) {
+          src[moves + __popc(ms & before)] = r;
+        } else if (r >= n && r < r_end) {  // (a moved row's are cleared once they are copied)
+          w[r] = 0.f;
+          tok[r] = -1;
+        }
       }
       holes += __popc(hs);
       moves += __popc(ms);
@@ -295,29 +335,26 @@ __global__ void __launch_bounds__(kEvThreads) kv_evict_select_kernel(const Evict
       }
     }
   }
-  cluster_sync(ranks);  // the lists are there
-  const int first = rank * threads + tid, step = ranks * threads;
-  for (int i = first; i < n_moves; i += step) {
-    const int s = src[i], d = dst[i];
-    w[d] = w[s];
-    tok[d] = tok[s];
-  }
-  cluster_sync(ranks);  // and the moved rows' weights and tokens were read
-#pragma unroll 4
-  for (int r = n + first; r < len; r += step) {
-    w[r] = 0.f;
-    tok[r] = -1;
-  }
+  cluster_sync(ranks);  // every CTA's words were read
 }
 
 // grid (ceil(cap / 32), B * nkv): half a warp copies one 256-byte K row and
-// one V row; the CTA's 32 rows are all loaded before the first store.
+// one V row, with the row's weight and token, which are cleared where they were;
+// the CTA's 32 rows are all loaded before the first store.
 __global__ void __launch_bounds__(256) kv_evict_move_kernel(const EvictArgs a, __nv_bfloat16* k_cache,
                                                             __nv_bfloat16* v_cache) {
   griddep_wait();
   griddep_launch_dependents();
   const int b = blockIdx.y / a.nkv, kvh = blockIdx.y % a.nkv;
   const int32_t* plan = a.plan + size_t(blockIdx.y) * (2 + 2 * size_t(a.cap));
+  const int sub = threadIdx.x >> 4, c = threadIdx.x & 15;
+  int from[2], to[2];  // read beside the number of moves; past it they are not used
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int idx = blockIdx.x * kEvMoveRows + i * 16 + sub;
+    from[i] = idx < a.cap ? plan[2 + idx] : 0;
+    to[i] = idx < a.cap ? plan[2 + a.cap + idx] : 0;
+  }
   const int moves = plan[0];
   if (moves < 0) return;
   if (blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0) {
@@ -326,26 +363,27 @@ __global__ void __launch_bounds__(256) kv_evict_move_kernel(const EvictArgs a, _
   }
   const int slot = a.cache_slot ? a.cache_slot[b] : b;
   const size_t head = (size_t(slot) * a.nkv + kvh) * a.max_seq;
-  const int sub = threadIdx.x >> 4, c = threadIdx.x & 15;
+  // lane 0 of a row also carries its weight, lane 1 its token
+  int32_t* words = (c == 0 ? reinterpret_cast<int32_t*>(a.weights) : a.tokens) + head;
   uint4 kr[2], vr[2];
-  int d[2];
+  int word[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int idx = blockIdx.x * kEvMoveRows + i * 16 + sub;
-    d[i] = -1;
-    if (idx < moves) {
-      const size_t s = head + plan[2 + idx];
-      d[i] = plan[2 + a.cap + idx];
-      kr[i] = reinterpret_cast<const uint4*>(k_cache + s * kAttnD)[c];
-      vr[i] = reinterpret_cast<const uint4*>(v_cache + s * kAttnD)[c];
-    }
+    if (blockIdx.x * kEvMoveRows + i * 16 + sub >= moves) continue;
+    kr[i] = reinterpret_cast<const uint4*>(k_cache + (head + from[i]) * kAttnD)[c];
+    vr[i] = reinterpret_cast<const uint4*>(v_cache + (head + from[i]) * kAttnD)[c];
+    if (c < 2) word[i] = words[from[i]];
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (d[i] >= 0) {
-      reinterpret_cast<uint4*>(k_cache + (head + d[i]) * kAttnD)[c] = kr[i];
-      reinterpret_cast<uint4*>(v_cache + (head + d[i]) * kAttnD)[c] = vr[i];
+  for (int i = 0; i < 2; ++i) {
+    if (blockIdx.x * kEvMoveRows + i * 16 + sub >= moves) continue;
+    reinterpret_cast<uint4*>(k_cache + (head + to[i]) * kAttnD)[c] = kr[i];
+    reinterpret_cast<uint4*>(v_cache + (head + to[i]) * kAttnD)[c] = vr[i];
+    if (c < 2) {
+      words[to[i]] = word[i];
+      words[from[i]] = c == 0 ? 0 : -1;  // (0.f is all zero bits)
     }
+  }
 }
 
 }  // namespace qmoe
