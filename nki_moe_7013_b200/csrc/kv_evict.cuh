@@ -12,9 +12,15 @@
 //
 // kv_evict_select_kernel (a cluster of one to eight CTAs per (sequence, KV
 // head), each holding a run of its rows) finds the n-th largest of the 32-bit
-// order keys eight bits at a time, lists the moves, and moves
-// the rows' weights and tokens; kv_evict_move_kernel copies the K and V rows
-// over all SMs and sets the new lengths.
+// order keys eight bits at a time, lists the moves and clears the weights and
+// tokens of the rows that go; kv_evict_move_kernel copies the kept rows with
+// theirs over all SMs and sets the new lengths.
+//
+// Bound by latency: the selection is a chain of short passes (lengths, the
+// newest token, two to four digits, ranks, the lists) of some 1,500 to 5,000
+// cycles each, a barrier of the CTA or its cluster after every one, and the
+// move waits for it.  8 sequences of 2,176 rows to 2,048 take 15.9 us, 4 of
+// up to 16,384 to 2,048 (28 MB moved) 23.6.
 #pragma once
 
 #include "attn_shared.cuh"

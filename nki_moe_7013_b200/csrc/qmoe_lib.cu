@@ -1913,13 +1913,17 @@ int qmoe_kv_evict(void* k_cache, void* v_cache, float* weights, int32_t* tokens,
   a.recent = int(recent);
   a.cap = int(std::min(keep, max_len));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // A cluster per (sequence, KV head) while the CTAs still fit the SMs at once
-  // and each holds 2,048 rows or more (measured with the move: 16,384 rows of
-  // 16 heads 38 us with one CTA each, 27 us with eight; 2,176 rows of 32 heads
-  // 17 us with one, 20 us with four), and about four rows per thread (more
-  // threads lengthen the barriers: 39 us at two rows per thread).
+  // A cluster per (sequence, KV head) while the CTAs still fit the SMs at once,
+  // from 4,096 rows on and 1,024 or more a CTA; about four rows per thread.
+  // Measured, with the move and with the copy that restores the cache between
+  // calls: 16,384 rows of 16 heads 35.0 us with one CTA each, 29.3 with two,
+  // 24.0 with four, 23.5 with eight; 4,352 rows of 16 heads 19.7 with one, 17.6
+  // with four; 2,176 rows of 32 heads 15.9 with one, 17.0 with four; two rows
+  // per thread 33.0 us for the first of these, eight 26.2.
   int cluster = 1, threads = 128;
-  while (cluster < qmoe::kEvMaxCluster && B * nkv * cluster * 2 <= d->sms && max_len >= 4096 * cluster) cluster *= 2;
+  while (cluster < qmoe::kEvMaxCluster && B * nkv * cluster * 2 <= d->sms &&
+         max_len >= std::max<int64_t>(4096, 2048 * cluster))
+    cluster *= 2;
   while (threads < qmoe::kEvThreads && max_len > 4 * threads * cluster) threads *= 2;
   a.cached = int(std::min<int64_t>(((max_len + cluster - 1) / cluster + 31) / 32 * 32, qmoe::kEvMaxCached));
   const int smem = a.cached * 4;
