@@ -9,9 +9,11 @@
 // diagonal crosses few of them.
 //
 // The prefix part of a decode step (kPartial true): the rows are the B * G
-// (sequence, head) rows of one KV head, so the prefix is read once for up to
-// 256 of them; the keys are cut into parts whose running maximum, sum and
-// unnormalised output go to shared_decode_combine_kernel.
+// (sequence, head) rows of one KV head, so the prefix is read once for 128 of
+// them (with kSplit) or 256; the keys are cut into parts whose running maximum,
+// sum and unnormalised output go to shared_decode_combine_kernel.  128
+// sequences on 16,384 rows: 22 steps on 96 SMs, 42 us, the tensor pipe 52 %
+// busy, the own rows' kernel on the other SMs beside it.
 //
 // One CTA = two softmax groups A and B; 320 threads: warps 0-3 and 4-7 softmax
 // (a thread owns a row = a TMEM lane), warp 8 the TMA producer (Q once, then K
@@ -20,8 +22,9 @@
 //   S_A(0) S_B(0) | PV_A(0) S_A(1) | PV_B(0) S_B(1) | PV_A(1) S_A(2) | ...
 // Without kSplit A and B are two row tiles sharing every K / V tile; with it
 // they are the even and the odd key tiles of one row tile, joined at the end
-// (each thread reads both groups' O of its TMEM lane): half the steps, for twice the CTAs, where the row tiles are
-// too few to fill the SMs.  S and O stay in TMEM (512 columns); P goes to
+// (each thread reads both groups' O of its TMEM lane): half the steps, for twice
+// the CTAs, where the row tiles are too few to fill the SMs, or half the parts
+// of a decode step.  S and O stay in TMEM (512 columns); P goes to
 // shared memory in bf16.  A row's O is rescaled only when its maximum grew by
 // more than 2^8.
 //

@@ -101,6 +101,12 @@ DECODE = [
     (9, 64, 4, 6016, [150] * 9, None, [8, 7, 6, 5, 4, 3, 2, 1, 0], 0),
     (12, 8, 1, 33000, [0] * 11 + [1], None, None, 0),          # 96 rows of one KV head: the keys split
     (130, 8, 8, 4000, [1] * 130, None, None, 0),
+    (20, 32, 4, 3000, [0] * 20, None, None, 0),                # nothing but the prefix
+    (300, 64, 4, 1200, [b % 41 for b in range(300)], None, None, 0),  # row tiles that share a CTA
+    (200, 64, 4, 1100, [40 - b % 7 for b in range(200)], None, None, 0),
+    # several row tiles that stay on the warp-level kernel
+    (8, 32, 4, 700, [400, 3, 77, 0, 128, 129, 399, 1], None, None, 0),
+    (7, 20, 4, 900, [333, 0, 64, 65, 300, 2, 1], [30, 0, 64, 1, 0, 2, 0], None, 0),
 ]
 
 
