@@ -1043,9 +1043,13 @@ SharedDecodePlan shared_decode_plan(int64_t B, int64_t G, int64_t nkv, int64_t P
     p.psplits = (P + p.pchunk - 1) / p.pchunk;
   }
   if (max_len > 0) {
-    // two CTAs per SM; every sequence has a part of its own, none shorter than
-    // 128 rows but its last.  Sequences that fill the SMs are not cut.
-    p.own_slots = B * nkv >= 2 * sms ? 0 : std::max<int64_t>(1, 2 * sms / nkv);
+    // two CTAs per SM, or one beside the tcgen05 kernel, which holds most SMs for
+    // most of the time (32 sequences of up to 700 rows on 2,048: two 20.7 us, one
+    // 18.6; 16 of 4,000 on 2,048 30.9 and 26.5; without a prefix 4 of 4,096 14.1
+    // and 15.4); every sequence has a part of its own, none shorter than 128 rows
+    // but its last.  Sequences that fill the SMs so are not cut.
+    const int64_t fill = p.tc ? sms : 2 * sms;
+    p.own_slots = B * nkv >= fill ? 0 : std::max<int64_t>(1, fill / nkv);
     p.own_cap = p.own_slots == 0 ? B : std::min(p.own_slots + B, B * ((max_len + 127) / 128));
   }
   // more parts (of an even batch) than two rounds of a warp's eight loads,
