@@ -1530,7 +1530,8 @@ int qmoe_qk_norm_rope_rows(const void* qkv, const int32_t* positions, const int3
   QMOE_CHECK(device_info(&d));
   if (T == 0) return QMOE_OK;
   // a CTA per token, each warp several heads
-  return launch_kernel(qmoe::qk_norm_rope_kernel, dim3(unsigned(T)), dim3(32 * qmoe::kQkWarps), 0,
+  return launch_kernel(cache_rows || row_tokens ? qmoe::qk_norm_rope_kernel<true> : qmoe::qk_norm_rope_kernel<false>,
+                       dim3(unsigned(T)), dim3(32 * qmoe::kQkWarps), 0,
                        static_cast<cudaStream_t>(stream), true, "qk_norm_rope_kernel",
                        static_cast<const __nv_bfloat16*>(qkv), positions, cache_slot, q_norm_w, k_norm_w, inv_freq,
                        int(T), int(nh), int(nkv), eps, static_cast<__nv_bfloat16*>(q_out),
