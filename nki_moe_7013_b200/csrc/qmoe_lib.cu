@@ -1049,7 +1049,11 @@ SharedDecodePlan shared_decode_plan(int64_t B, int64_t G, int64_t nkv, int64_t P
     // and 15.4); every sequence has a part of its own, none shorter than 128 rows
     // but its last.  Sequences that fill the SMs so are not cut.
     const int64_t fill = p.tc ? sms : 2 * sms;
-    p.own_slots = B * nkv >= fill ? 0 : std::max<int64_t>(1, fill / nkv);
+    // Each sequence's last part is short, about half a one a sequence too many:
+    // alone on the SMs that would be a second wave, so fewer are aimed at (32
+    // sequences of up to 2,000 rows, with weights, 30.7 and 27.3 us, 16 of 9,000
+    // 55.3 and 51.8; beside the prefix part 16 of 4,000 26.4 and 28.1).
+    p.own_slots = B * nkv >= fill ? 0 : std::max(B, fill / nkv - (p.tc ? 0 : B / 2));
     p.own_cap = p.own_slots == 0 ? B : std::min(p.own_slots + B, B * ((max_len + 127) / 128));
   }
   // more parts (of an even batch) than two rounds of a warp's eight loads,
