@@ -238,8 +238,16 @@ __global__ void __launch_bounds__(kAwThreads, 1)
 #pragma unroll
           for (int g = 0; g < kAwTiles; ++g) {
             if (g >= tiles || !ok) continue;
+            // The place's last use must be done.  A parity wait also passes on
+            // a barrier two phases behind, and the slots take turns at loading:
+            // with units of one query tile the use before the last may still
+            // run, so k_empty alone will not do.  First the last use's tile must
+            // have landed: it was loaded once the use before was done.  The uses
+            // before that have landed, since the q_empty waited for above
+            // follows them (below).
             ok = used[g] == 0 ||
-                 fa_wait_warp(&k_empty[g], (used[g] - 1) & 1, abort_flag, kDevErrWaitTimeoutProducer);
+                 (fa_wait_warp(&k_full[g], (used[g] - 1) & 1, abort_flag, kDevErrWaitTimeoutProducer) &&
+                  fa_wait_warp(&k_empty[g], (used[g] - 1) & 1, abort_flag, kDevErrWaitTimeoutProducer));
             if (ok && lane == 0) {
               const int z = blk.slot * a.nkv + kvh, y = blk.key0 + g * kFaRows;
               loads[kAwSlots + g] = used[g] + 1;
@@ -305,9 +313,9 @@ __global__ void __launch_bounds__(kAwThreads, 1)
                          q_desc + ((sl * kFaTileBytes) >> 4), idesc);
           umma_commit(&s_full[g]);
         }
-        umma_commit(&q_empty[sl]);
-        // the unit's K tiles are free once these products are done; one that
-        // no query of the chunk saw must have landed first
+        // The unit's K tiles are free once these products are done; one that
+        // no query of the chunk saw must have landed first.  All this before
+        // q_empty, on which a slot takes the unit's K tiles as landed.
         if (flags & kAwLast) {
 #pragma unroll
           for (int g = 0; g < kAwTiles; ++g) {
@@ -318,6 +326,7 @@ __global__ void __launch_bounds__(kAwThreads, 1)
             ++units[g];
           }
         }
+        umma_commit(&q_empty[sl]);
       }
       umma_commit(drain);
       const unsigned long long start = globaltimer_ns();

@@ -1,0 +1,65 @@
+"""Shared-prefix and bounded-cache operators on batches that make a CTA, a
+kernel form or a padding meet more than one sequence, against 64 bits."""
+import pytest
+import torch
+
+from test_shared_attention_gpu import C, HD, _check_weights, _error, _gen, _i32, _randn
+
+pytestmark = pytest.mark.gpu
+
+
+def _prompt_weights(B, nh, nkv, S, past, pads, accumulate, seed):
+    """The totals of a call next to those in 64 bits.  The log-sum-exp handed
+    over is the 64-bit one rounded to fp32: off by at most 2^-24 of itself,
+    which the score's 136 * 2^-24 * D of _check_weights' second delta covers
+    (|lse| <= D + ln L, L <= 4096, and D > 5 for these inputs)."""
+    from nki_moe_7013_b200 import ops
+
+    g = _gen(seed)
+    G, L = nh // nkv, past + S
+    k, q = _randn(g, B, nkv, L + 3, HD), _randn(g, B * S, nh, HD)
+    k[:, :, L:] = float("nan")
+    w = torch.rand(B, nkv, L + 3, generator=g, device="cuda")
+    before = w.double()
+    add = torch.zeros_like(before)
+    lse = torch.full((B, S, nh), float("-inf"), device="cuda")
+    pos, D = past + torch.arange(S, device="cuda"), 0.0
+    for b in range(B):
+        lo = min(pads[b], L)
+        k[b, :, :lo] = float("nan")
+        if not accumulate:
+            before[b, :, :L] = 0
+        if lo == L:
+            continue
+        qd = q[b * S:(b + 1) * S].double().view(S, nkv, G, HD).permute(1, 2, 0, 3)  # nkv, G, S
+        kd = k[b, :, lo:L].double()
+        s = torch.matmul(qd, kd[:, None].transpose(2, 3)) * C
+        D = max(D, float((torch.matmul(qd.abs(), kd.abs()[:, None].transpose(2, 3)) * C).max()))
+        s.masked_fill_(torch.arange(lo, L, device="cuda")[None] > pos[:, None], float("-inf"))
+        row = torch.logsumexp(s, dim=3)
+        lse[b] = row.permute(2, 0, 1).reshape(S, nh)
+        live = row > float("-inf")
+        p = torch.where(live[..., None], torch.exp(s - torch.where(live, row, 0.0)[..., None]), 0.0)
+        add[b, :, lo:L] = p.sum(dim=(1, 2))
+    assert D > 5
+    ops.attention_weights(q, lse.view(B * S, nh), k, _i32([past] * B), B, S, w, accumulate=accumulate,
+                          kv_start=_i32(pads))
+    assert _error() == 0
+    _check_weights(w, add, before, D)
+
+
+@pytest.mark.parametrize("S,nh", [(1, 32), (4, 32), (16, 32), (16, 20), (17, 32)])
+def test_prompt_weights_of_many_short_units(cuda_dev, S, nh):
+    """64 sequences, four key blocks each: a CTA takes seven units in turn, most
+    of one query tile (17 queries of 8 heads: two)."""
+    B, past = 64, 2001
+    _prompt_weights(B, nh, 4, S, past, [37 * b if b % 3 else 0 for b in range(B)], S % 2 == 0, seed=S)
+
+
+@pytest.mark.parametrize("B,nh,nkv,S,past,pads", [
+    (3, 16, 2, 2000, 500, [0, 700, 2400]),   # chunks of five query tiles, four units a CTA and more
+    (40, 32, 4, 70, 1100, [30 * b for b in range(40)]),  # chunks of units, some sequences nearly all padding
+    (1, 8, 8, 4000, 0, [1]),
+])
+def test_prompt_weights_of_many_units(cuda_dev, B, nh, nkv, S, past, pads):
+    _prompt_weights(B, nh, nkv, S, past, pads, False, seed=B)
