@@ -479,8 +479,9 @@ QMOE_API int qmoe_attention_decode(const void* q, const void* k_cache, const voi
  * qmoe_attention_prefix_decode: one query per sequence, q (B, nh, 128) bf16,
  *   over the prefix and own rows up to kv_len[b] - 1 (kv_len[b] <= max_len;
  *   0 allowed).  A query that sees no row gets zeros.  weights NULL: none.
- *   workspace: _workspace_size() bytes (may be 0), 256-byte aligned, any
- *   contents; calls that share one must not overlap on the GPU.
+ *   workspace: _workspace_size() bytes (may be 0; 0 also for a shape that the
+ *   call refuses), 256-byte aligned, any contents; calls that share one must
+ *   not overlap on the GPU.
  * qmoe_attention_prefix_prefill: S queries per sequence, q (B*S, nh, 128);
  *   query i sees the prefix and own rows up to q_start[b] + i.  A query
  *   before kv_start (a padding position) gets a zero row.  lse (B*S, nh) fp32

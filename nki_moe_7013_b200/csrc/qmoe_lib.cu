@@ -1093,6 +1093,13 @@ AttnWeightsPlan attn_weights_plan(int64_t B, int64_t S, int64_t G, int64_t nkv, 
   return p;
 }
 
+// Heads that the shared-attention kernels take: the size queries answer 0 to
+// others (the plans divide by the rows of a tile per group), and the entry
+// points refuse them by name.
+bool shared_heads_ok(int64_t nh, int64_t nkv) {
+  return nh > 0 && nkv > 0 && nh % nkv == 0 && nh / nkv <= qmoe::kSdMaxGroup;
+}
+
 int check_shared_attention(const char* what, int64_t head_dim, int64_t nh, int64_t nkv, int64_t n_slots,
                            int64_t max_seq, float scale) {
   QMOE_REQUIRE(head_dim == qmoe::kAttnD, QMOE_ERR_UNSUPPORTED_SHAPE, "%s: head_dim must be 128", what);
@@ -1654,7 +1661,7 @@ int qmoe_attention_decode(const void* q, const void* k_cache, const void* v_cach
 
 size_t qmoe_attention_prefix_decode_workspace_size(int64_t B, int64_t nh, int64_t nkv, int64_t prefix_len,
                                                    int64_t max_len, int with_weights) {
-  if (B <= 0 || nkv <= 0 || nh <= 0 || nh % nkv != 0 || prefix_len < 0 || max_len < 0) return 0;
+  if (B <= 0 || !shared_heads_ok(nh, nkv) || prefix_len < 0 || max_len < 0) return 0;
   return shared_decode_bytes(shared_decode_plan(B, nh / nkv, nkv, prefix_len, max_len), B, nh, max_len,
                              with_weights != 0);
 }
@@ -1819,7 +1826,7 @@ int qmoe_attention_prefix_prefill(const void* q, const void* k_prefix, const voi
 }
 
 size_t qmoe_attention_weights_workspace_size(int64_t B, int64_t S, int64_t nh, int64_t nkv, int64_t max_len) {
-  if (B <= 0 || S <= 0 || nkv <= 0 || nh <= 0 || nh % nkv != 0 || max_len <= 0) return 0;
+  if (B <= 0 || S <= 0 || !shared_heads_ok(nh, nkv) || max_len <= 0) return 0;
   const AttnWeightsPlan p = attn_weights_plan(B, S, nh / nkv, nkv, max_len);
   return p.chunks > 1 ? size_t(p.chunks * B * nkv * p.key_blocks) * qmoe::kAwKeys * sizeof(float) : 0;
 }

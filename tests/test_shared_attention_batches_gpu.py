@@ -63,3 +63,20 @@ def test_prompt_weights_of_many_short_units(cuda_dev, S, nh):
 ])
 def test_prompt_weights_of_many_units(cuda_dev, B, nh, nkv, S, past, pads):
     _prompt_weights(B, nh, nkv, S, past, pads, False, seed=B)
+
+
+@pytest.mark.parametrize("nh,nkv", [(34, 2), (17, 1), (256, 1)])
+def test_unsupported_head_ratios_are_refused(cuda_dev, nh, nkv):
+    """More than 16 query heads per KV head: a named error from the wrappers."""
+    from nki_moe_7013_b200 import _C, ops
+
+    bf = dict(dtype=torch.bfloat16, device="cuda")
+    k, q = torch.zeros(2, nkv, 600, HD, **bf), torch.zeros(2, nh, HD, **bf)
+    n, w = _i32([3, 4]), torch.zeros(2, nkv, 600, device="cuda")
+    for call in (lambda: ops.attention_prefix_decode(q, k, k, 600, k, k, n, 600),
+                 lambda: ops.attention_decode_weights(q, k, k, n, 600, w),
+                 lambda: ops.attention_prefix_prefill(q, k, k, 600, k, k, n, 2, 1),
+                 lambda: ops.attention_weights(q, torch.zeros(2, nh, device="cuda"), k, n, 2, 1, w)):
+        with pytest.raises(_C.QmoeError, match="query heads per KV head"):
+            call()
+    assert _error() == 0 and not w.any()
