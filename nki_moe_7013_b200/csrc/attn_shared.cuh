@@ -539,16 +539,18 @@ struct RowParts {
                                             lane * 4);
   }
 };
-// (A sequence without own rows has no part that wrote its plan.)
 __device__ __forceinline__ RowParts row_parts(const SharedDecodeArgs& a, int own_count, int own_first, int b, int h) {
   const size_t bh = size_t(b) * a.nh + h, first = size_t(own_first) * a.nh + h;
   return {a.pre_ml + bh * a.psplits * 2, a.pre_o + bh * a.psplits * kAttnD, a.own_ml + first * 2,
           a.own_o + first * kAttnD,      a.psplits, a.psplits + own_count,  a.nh};
 }
-__device__ __forceinline__ int2 own_plan(const SharedDecodeArgs& a, int b) {
-  if (a.max_len == 0) return make_int2(0, 0);
+// A sequence's first own part and their number; one without own rows has no
+// part that wrote its plan.  `ok` as of own_range.
+__device__ __forceinline__ int2 own_plan(const SharedDecodeArgs& a, int b, bool& ok) {
+  int slot, lo, hi;
   const int2 p = a.plan[b];
-  return own_rows(a, b) > 0 ? p : make_int2(0, 0);
+  ok = own_range(a.kv_len, a.cache_slot, a.kv_start, b, a.max_len, a.n_slots, slot, lo, hi);
+  return hi > lo ? p : make_int2(0, 0);
 }
 
 // M and 1/l of one row from its parts, in every lane of the warp.
@@ -586,7 +588,11 @@ __global__ void __launch_bounds__(256) shared_decode_combine_kernel(const Shared
     const int gw = a.wide ? blockIdx.x : blockIdx.x * 8 + warp;
     if (gw >= a.B * a.nh) return;
     const int b = gw / a.nh;
-    const int2 own = own_plan(a, b);
+    bool ok;
+    const int2 own = own_plan(a, b, ok);
+    // (where own rows are cut, a sequence whose length or slot lies outside the
+    // cache has no part that could report it)
+    if (!ok && gw % a.nh == 0 && lane == 0 && (!a.wide || warp == 0)) record_device_error(kDevErrBadIndex);
     const RowParts p = row_parts(a, own.y, own.x, b, gw % a.nh);
     float M, inv;
     join_ml(p, lane, M, inv);
@@ -638,7 +644,7 @@ __global__ void __launch_bounds__(256) shared_decode_combine_kernel(const Shared
   const int rb = v % a.row_blocks, rest = v / a.row_blocks;
   const int kvh = rest % a.nkv, b = rest / a.nkv;
   int slot, lo, hi;
-  if (!own_range(a.kv_len, a.cache_slot, a.kv_start, b, a.max_len, a.n_slots, slot, lo, hi)) return;  // recorded before
+  if (!own_range(a.kv_len, a.cache_slot, a.kv_start, b, a.max_len, a.n_slots, slot, lo, hi)) return;  // (reported above)
   const int first = rb * kSdCombineRows;
   if (first >= hi) return;
   const int row = first + threadIdx.x;
@@ -649,7 +655,8 @@ __global__ void __launch_bounds__(256) shared_decode_combine_kernel(const Shared
 #pragma unroll
   for (int h = 0; h < kSdMaxGroup; ++h) sc[h] = h < a.G && row >= lo && row < hi ? sp[h] : -INFINITY;
   const float total = a.accumulate && row < hi ? *dst : 0.f;
-  const int2 own = own_plan(a, b);
+  bool ok;
+  const int2 own = own_plan(a, b, ok);
   for (int h = warp; h < a.G; h += 8) {
     float M, inv;
     join_ml(row_parts(a, own.y, own.x, b, kvh * a.G + h), lane, M, inv);

@@ -80,3 +80,45 @@ def test_unsupported_head_ratios_are_refused(cuda_dev, nh, nkv):
         with pytest.raises(_C.QmoeError, match="query heads per KV head"):
             call()
     assert _error() == 0 and not w.any()
+
+
+# (B, nkv, prefix, max_len): cut own rows, uncut ones, a prefix in parts of the
+# warp-level kernel, on the tcgen05 kernel with cut and uncut own rows, rows of
+# many parts, one kernel, no own rows
+PATHS = [(3, 4, 0, 700), (74, 4, 0, 1100), (3, 4, 600, 90), (20, 4, 3001, 90), (40, 4, 3001, 90), (2, 4, 5000, 9000),
+         (3, 4, 70, 90), (3, 4, 600, 0), (20, 4, 3001, 0)]
+
+
+def _batch(B, nkv, P, max_len):
+    g = _gen(P + max_len)
+    k, v = _randn(g, B, nkv, max_len + 8, HD), _randn(g, B, nkv, max_len + 8, HD)
+    kp, vp = _randn(g, 1, nkv, max(P, 1), HD), _randn(g, 1, nkv, max(P, 1), HD)
+    lens = [max(0, max_len - 3 * b) for b in range(B)]
+    return k, v, kp, vp, _randn(g, B, 8 * nkv, HD), lens
+
+
+@pytest.mark.parametrize("path", PATHS)
+def test_decode_reports_bad_lengths_and_slots(cuda_dev, path):
+    """A length past max_len or below 0, or a slot outside the cache: device
+    error 4 whatever form the call takes, and what a sequence without own rows
+    gives; the others' outputs and weights as ever."""
+    from nki_moe_7013_b200 import ops
+
+    B, nkv, P, max_len = path
+    k, v, kp, vp, q, lens = _batch(*path)
+    bad = B - 1
+    empty = lens[:bad] + [0]
+
+    def call(lens, slots, weights):
+        w = torch.full((B, nkv, max_len + 8), 0.5, device="cuda") if weights else None
+        out = ops.attention_prefix_decode(q, kp, vp, P, k, v, _i32(lens), max_len, cache_slot=_i32(slots), weights=w)
+        return out, w
+
+    for weights in (False, True):
+        want, want_w = call(empty, None, weights)
+        assert _error() == 0
+        for length, slot in ((max_len + 1, bad), (-1, bad), (min(5, max_len), B), (min(5, max_len), -1)):
+            out, w = call(lens[:bad] + [length], list(range(bad)) + [slot], weights)
+            assert _error() == 4, (length, slot, weights)
+            assert torch.equal(out, want)
+            assert w is None or torch.equal(w, want_w)
