@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(256) shared_decode_combine_kernel(const Shared
   int slot, lo, hi;
   if (!own_range(a.kv_len, a.cache_slot, a.kv_start, b, a.max_len, a.n_slots, slot, lo, hi)) return;  // (reported above)
   const int first = rb * kSdCombineRows;
-  if (first >= hi) return;
+  if (first >= hi && rb > 0) return;  // (the first block also looks for a slot given twice)
   const int row = first + threadIdx.x;
   // the row's scores and total, in flight while the maxima are joined
   const float* sp = a.scores + (size_t(b * a.nkv + kvh) * a.score_rows + row) * a.G;

@@ -1754,7 +1754,7 @@ int qmoe_attention_prefix_decode(const void* q, const void* k_prefix, const void
   a.score_rows = int(max_len);
   a.wide = p.wide ? 1 : 0;
   a.n_out_blocks = int(p.wide ? B * nh : (B * nh + 7) / 8);
-  a.row_blocks = int((max_len + qmoe::kSdCombineRows - 1) / qmoe::kSdCombineRows);
+  a.row_blocks = int(std::max<int64_t>(1, (max_len + qmoe::kSdCombineRows - 1) / qmoe::kSdCombineRows));
   a.direct = p.direct ? 1 : 0;
   a.overlaps = p.tc ? 1 : 0;
   a.scale_log2 = scale * 1.4426950408889634f;

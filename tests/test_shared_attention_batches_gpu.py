@@ -122,3 +122,24 @@ def test_decode_reports_bad_lengths_and_slots(cuda_dev, path):
             assert _error() == 4, (length, slot, weights)
             assert torch.equal(out, want)
             assert w is None or torch.equal(w, want_w)
+
+
+@pytest.mark.parametrize("path", PATHS)
+def test_decode_reports_a_slot_given_twice(cuda_dev, path):
+    """Weights of two entries of one slot: device error 4 and the first entry's
+    weights alone, also where one of the two holds no own rows."""
+    from nki_moe_7013_b200 import ops
+
+    B, nkv, P, max_len = path
+    k, v, kp, vp, q, lens = _batch(*path)
+    for first, second in ((lens[0], lens[1]), (lens[0], 0), (0, lens[1])):
+        n = [first, second] + lens[2:]
+        w = torch.zeros(B, nkv, max_len + 8, device="cuda")
+        slots = list(range(B))
+        ops.attention_prefix_decode(q, kp, vp, P, k, v, _i32(n), max_len, cache_slot=_i32(slots), weights=w)
+        assert _error() == 0
+        twice = torch.zeros_like(w)
+        slots[1] = 0
+        ops.attention_prefix_decode(q, kp, vp, P, k, v, _i32(n), max_len, cache_slot=_i32(slots), weights=twice)
+        assert _error() == 4, (first, second)
+        assert torch.equal(twice[0], w[0]) and not twice[1].any() and torch.equal(twice[2:], w[2:])
