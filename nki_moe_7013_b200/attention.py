@@ -333,7 +333,10 @@ class Qwen3MoeAttention(nn.Module):
                                  cache.k, cache.v, cache_slot=slots, cache_rows=rows_dev, row_tokens=cache.tokens,
                                  row_weights=cache.weights)
         kp, vp, pslot = (prefix.k, prefix.v, prefix.slot) if P else (None, None, 0)
-        if S == 1:
+        # The decode kernels do not know a query that is itself a padding: it
+        # would see the prefix.  The prefill gives it zeros.
+        padding = P > 0 and any(p > l for p, l in zip(pad_now, L0))
+        if S == 1 and not padding:
             kv_len = torch.tensor([l + 1 for l in L0], dtype=torch.int32).to(dev, non_blocking=True)
             if apart:
                 with stage(timer, "attention"):

@@ -143,3 +143,30 @@ def test_decode_reports_a_slot_given_twice(cuda_dev, path):
         ops.attention_prefix_decode(q, kp, vp, P, k, v, _i32(n), max_len, cache_slot=_i32(slots), weights=twice)
         assert _error() == 4, (first, second)
         assert torch.equal(twice[0], w[0]) and not twice[1].any() and torch.equal(twice[2:], w[2:])
+
+
+def test_one_padding_token_behind_a_prefix(cuda_dev):
+    """Prompts fed a token at a time, the second sequence's first two tokens
+    paddings: zero rows for these, and each sequence as if it were run whole."""
+    from helpers import MAX_REL, activations, max_rel_err, to_f32_np
+    from nki_moe_7013_b200.attention import Qwen3MoeAttention
+    from nki_moe_7013_b200.config import Qwen3MoeConfig
+
+    cfg = Qwen3MoeConfig()
+    attn, H = Qwen3MoeAttention(cfg, device=cuda_dev, seed=13), cfg.hidden_size
+    P, B, S, pads = 21, 2, 5, [0, 2]
+    xp = activations(21, P, H, cuda_dev).view(1, P, H)
+    x = activations(22, B * S, H, cuda_dev).view(B, S, H)
+    prefix = attn(xp)[1].as_prefix()
+    for track in (False, True):
+        cache = attn.new_cache(B, S, track=track)
+        mask = (torch.arange(S)[None] >= torch.tensor(pads)[:, None]).int()
+        got = torch.cat([attn(x[:, i:i + 1], None, cache, attention_mask=mask[:, :i + 1], prefix=prefix)[0]
+                         for i in range(S)], dim=1)
+        for b in range(B):
+            assert not got[b, :pads[b]].any()
+            whole, _ = attn(torch.cat([xp, x[b:b + 1, pads[b]:]], dim=1))
+            assert max_rel_err(to_f32_np(got[b, pads[b]:]), to_f32_np(whole[0, P:])) <= MAX_REL
+        if track:
+            assert not cache.weights[1, :, :pads[1]].any()
+    assert _error() == 0
