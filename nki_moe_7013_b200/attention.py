@@ -35,6 +35,7 @@ flash-decode, their forms over a shared prefix, and the eviction.
 """
 from __future__ import annotations
 
+import copy
 from dataclasses import dataclass
 from typing import List, Optional
 
@@ -80,8 +81,18 @@ class KVCache:
     def _clear_positions(self, n_slots: int) -> None:
         self.offset: List[int] = [0] * n_slots      # a new row's position less the row
         self.prefix_len: List[int] = [0] * n_slots  # rows of the shared prefix the slot was filled behind
+        self.behind: List[Optional["SharedPrefix"]] = [None] * n_slots  # that prefix (None: none, or not known)
         self.lead: List[int] = [0] * n_slots        # leading paddings the slot was filled with
         self.dropped: List[int] = [0] * n_slots     # rows evicted so far
+
+    def __deepcopy__(self, memo) -> "KVCache":
+        # a copy stays behind the same prefix, which is not copied with it
+        for p in self.behind:
+            if p is not None:
+                memo.setdefault(id(p), p)
+        c = memo[id(self)] = object.__new__(type(self))
+        c.__dict__.update(copy.deepcopy(self.__dict__, memo))
+        return c
 
     @property
     def tracked(self) -> bool:
@@ -113,14 +124,18 @@ class KVCache:
         self._clear_positions(self.n_slots)
         return self
 
-    def _follow(self, prefix_len: int, pads: Optional[List[int]], B: int) -> None:
+    def _follow(self, prefix_len: int, pads: Optional[List[int]], B: int,
+                prefix: Optional["SharedPrefix"] = None) -> None:
         """The host's side of a call that appends to slots 0 .. B-1 behind
-        ``prefix_len`` shared rows: refuses what the rows already there
-        contradict, and records paddings (``pads``; None: as they are) and the
-        distance of a new row's position from the row."""
+        ``prefix_len`` shared rows (those of ``prefix``): refuses what the rows
+        already there contradict, and records paddings (``pads``; None: as they
+        are), the prefix and the distance of a new row's position from the row."""
         for b in range(B):
             fresh = self.lengths[b] == 0 and self.dropped[b] == 0
-            if not fresh and self.prefix_len[b] != prefix_len:
+            none_yet = self.dropped[b] == 0 and self.lengths[b] <= self.pad[b]
+            was = self.behind[b]
+            if not fresh and (self.prefix_len[b] != prefix_len or not (
+                    none_yet or was is None or prefix is None or was.same_rows(prefix))):
                 raise ValueError("the cache was filled behind another prefix (or none)")
             if prefix_len and pads is not None and pads[b] != self.pad[b] and pads[b] < self.lengths[b]:
                 raise ValueError("attention_mask: behind a prefix the paddings come with a sequence's first tokens")
@@ -130,6 +145,7 @@ class KVCache:
             if self.dropped[b] == 0 and self.lengths[b] <= self.pad[b]:  # no token yet
                 # behind a prefix the distance to it counts, so paddings are left out of the positions
                 self.prefix_len[b] = prefix_len
+                self.behind[b] = prefix if prefix_len else None
                 self.offset[b] = prefix_len - self.pad[b] if prefix_len else 0
 
     def as_prefix(self, slot: int = 0) -> "SharedPrefix":
@@ -171,12 +187,18 @@ class KVCache:
 class SharedPrefix:
     """Rows 0 .. length-1 of slot ``slot`` of a K / V cache (n, nkv, rows, 128)
     bf16, rotated for positions 0 .. length-1, that every sequence of a batch
-    sees before its own rows."""
+    sees before its own rows.  Caches filled behind it hold on to it: their
+    later calls take the same prefix, where it was."""
 
     k: torch.Tensor
     v: torch.Tensor
     length: int
     slot: int = 0
+
+    def same_rows(self, other: "SharedPrefix") -> bool:
+        """The same rows of the same memory (contents are not compared)."""
+        return (self.length == other.length and self.slot == other.slot and self.k.shape == other.k.shape
+                and self.k.data_ptr() == other.k.data_ptr() and self.v.data_ptr() == other.v.data_ptr())
 
 
 def left_padding(attention_mask: Optional[torch.Tensor], B: int, S: int, L0: List[int]) -> Optional[List[int]]:
@@ -305,7 +327,7 @@ class Qwen3MoeAttention(nn.Module):
             raise ValueError("the prefix's slot is one of the batch's own")
         if attention_mask is not None and any(cache.dropped[:B]):
             raise ValueError("attention_mask: the cache evicted rows (its paddings among them); pass no mask")
-        cache._follow(P, left_padding(attention_mask, B, S, L0), B)
+        cache._follow(P, left_padding(attention_mask, B, S, L0), B, prefix)
         pad_now = cache.pad[:B]
         rows = (torch.tensor(L0, dtype=torch.int32).unsqueeze(1) + torch.arange(S, dtype=torch.int32))
         pos = rows + torch.tensor(cache.offset[:B], dtype=torch.int32).unsqueeze(1)

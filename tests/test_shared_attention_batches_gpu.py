@@ -170,3 +170,22 @@ def test_one_padding_token_behind_a_prefix(cuda_dev):
         if track:
             assert not cache.weights[1, :, :pads[1]].any()
     assert _error() == 0
+
+
+def test_another_prefix_of_the_same_length_is_refused(cuda_dev):
+    from helpers import activations
+    from nki_moe_7013_b200.attention import Qwen3MoeAttention
+    from nki_moe_7013_b200.config import Qwen3MoeConfig
+
+    cfg = Qwen3MoeConfig()
+    attn, H = Qwen3MoeAttention(cfg, device=cuda_dev, seed=14), cfg.hidden_size
+    a, b = (attn(activations(s, 9, H, cuda_dev).view(1, 9, H))[1].as_prefix() for s in (31, 32))
+    x = activations(33, 8, H, cuda_dev).view(2, 4, H)
+    cache = attn.new_cache(2, 8)
+    attn(x, None, cache, prefix=a)
+    with pytest.raises(ValueError, match="another prefix"):
+        attn(x[:, :1], None, cache, prefix=b)
+    assert cache.lengths == [4, 4]
+    attn(x[:, :1], None, cache, prefix=a)
+    attn(x, None, cache.reset(), prefix=b)
+    assert _error() == 0
