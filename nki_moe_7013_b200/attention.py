@@ -327,6 +327,9 @@ class Qwen3MoeAttention(nn.Module):
             raise ValueError("the prefix's slot is one of the batch's own")
         if attention_mask is not None and any(cache.dropped[:B]):
             raise ValueError("attention_mask: the cache evicted rows (its paddings among them); pass no mask")
+        kept = None
+        if position_ids is not None:
+            kept = {name: list(getattr(cache, name)) for name in ("pad", "lead", "prefix_len", "behind", "offset")}
         cache._follow(P, left_padding(attention_mask, B, S, L0), B, prefix)
         pad_now = cache.pad[:B]
         rows = (torch.tensor(L0, dtype=torch.int32).unsqueeze(1) + torch.arange(S, dtype=torch.int32))
@@ -340,6 +343,7 @@ class Qwen3MoeAttention(nn.Module):
                 shifted = pos  # paddings are left out already
             real = rows >= torch.tensor(pad_now, dtype=torch.int32).unsqueeze(1)  # padding tokens may carry any position
             if not (torch.equal(given, pos) or bool(torch.all((given == shifted) | ~real))):
+                vars(cache).update(kept)  # a refused call is not remembered
                 raise ValueError("position_ids must continue each sequence's cache contiguously (or, with left "
                                  "padding, count from the first real token)")
         positions = pos.reshape(-1).to(dev, non_blocking=True)

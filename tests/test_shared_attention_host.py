@@ -79,3 +79,29 @@ def test_a_cache_stays_behind_its_prefix():
     d.lengths = [3]
     with pytest.raises(ValueError, match="another prefix"):
         d._follow(5, None, 1, a)
+
+
+@pytest.mark.parametrize("behind", [False, True])
+def test_refused_positions_leave_the_cache_as_it_was(behind):
+    """Positions that do not continue the cache: refused before anything runs,
+    and paddings of the refused call are not remembered."""
+    from nki_moe_7013_b200.attention import Qwen3MoeAttention
+
+    attn = object.__new__(Qwen3MoeAttention)
+    object.__setattr__(attn, "cfg", None)
+    prefix = _prefix() if behind else None
+    x = torch.zeros(2, 4, 8)
+    mask = torch.tensor([[1, 1, 1, 1], [0, 0, 1, 1]])
+    for lengths in ([0, 0], [4, 4]):
+        c = KVCache(2, 2, 16, 128, device="cpu")
+        if lengths[0]:
+            c._follow(5 if behind else 0, [0, 1], 2, prefix)
+            c.lengths, mask = lengths, torch.cat([torch.ones(2, 4, dtype=torch.int64), mask], dim=1)
+            mask[1, :4] = torch.tensor([0, 1, 1, 1])
+            mask[1, 4:] = 1
+            if not behind:
+                mask[1, 1] = 0  # without a prefix the paddings may change
+        kept = [list(getattr(c, n)) for n in ("pad", "lead", "prefix_len", "offset", "behind")]
+        with pytest.raises(ValueError, match="position_ids"):
+            Qwen3MoeAttention.forward(attn, x, torch.full((2, 4), 40), c, attention_mask=mask, prefix=prefix)
+        assert [getattr(c, n) for n in ("pad", "lead", "prefix_len", "offset", "behind")] == kept
