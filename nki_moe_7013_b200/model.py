@@ -252,6 +252,8 @@ class DecodeSession:
         if fill_random:
             for l, c in enumerate(self.caches):
                 c.fill_random(context, seed=seed * 100 + l)
+                if P:
+                    c.prefix_len, c.offset, c.behind = [P] * batch, [P] * batch, [prefix[l]] * batch
         for c in self.caches:
             if c.tracked:  # the tokens of the rows the caches are entered with
                 c.tokens[:, :, :context] = torch.arange(P, P + context, dtype=torch.int32, device=dev)
@@ -304,6 +306,8 @@ class DecodeSession:
 
     def step(self) -> torch.Tensor:
         """One decode step on the current stream (or the captured graph)."""
+        if self.steps_done == 0:
+            self._check_prefix()
         self._make_room()
         if self.graph is not None:
             self.graph.replay()
@@ -312,6 +316,15 @@ class DecodeSession:
         self.steps_done += 1
         self.rows_used += 1
         return self.tokens
+
+    def _check_prefix(self) -> None:
+        """Before the first step: caches that prompts have filled follow the
+        session's prefix (or none, like it)."""
+        for l, c in enumerate(self.caches):
+            px = self.prefix[l] if self.prefix else SharedPrefix(None, None, 0)
+            for n, length, was in zip(c.lengths, c.prefix_len, c.behind):
+                if n and (length != px.length or not (was is None or was.same_rows(px))):
+                    raise ValueError("the session's caches were filled behind another prefix (or none)")
 
     def _make_room(self) -> None:
         """Evict every layer's cache to ``keep`` rows when it is full."""
@@ -342,6 +355,8 @@ class DecodeSession:
         """Capture one step into a CUDA graph (run one eager step first so
         every kernel's attributes are set outside the capture)."""
         dev = self.model.device
+        if self.steps_done == 0:
+            self._check_prefix()
         self._make_room()
         s = torch.cuda.Stream(dev)
         s.wait_stream(torch.cuda.current_stream(dev))

@@ -189,3 +189,28 @@ def test_another_prefix_of_the_same_length_is_refused(cuda_dev):
     attn(x[:, :1], None, cache, prefix=a)
     attn(x, None, cache.reset(), prefix=b)
     assert _error() == 0
+
+
+def test_a_session_steps_behind_the_prefix_of_its_caches(cuda_dev):
+    """Prompts prefilled into a session's caches behind another prefix than the
+    session's, or behind none: refused before the first step."""
+    from nki_moe_7013_b200.config import Qwen3MoeConfig
+    from nki_moe_7013_b200.model import DecodeSession, Qwen3MoeModel
+
+    model = Qwen3MoeModel(Qwen3MoeConfig(), num_layers=1, vocab_size=512, device=cuda_dev, seed=15)
+    ids = torch.arange(40, device=cuda_dev)
+    a, b = model.prefill_prefix(ids[:20]), model.prefill_prefix(ids[20:])
+    for mine, other in ((a, b), (a, None), (None, a)):
+        for first in ("step", "capture"):
+            sess = DecodeSession(model, 2, context=6, max_new=4, prefix=mine, fill_random=False)
+            model.forward(ids[:12].view(2, 6), sess.caches, prefix=other)
+            with pytest.raises(ValueError, match="another prefix"):
+                getattr(sess, first)()
+            assert sess.steps_done == 0
+        for c in sess.caches:
+            c.reset()
+        model.forward(ids[:12].view(2, 6), sess.caches, prefix=mine)
+        sess.step()
+        sess.step()
+        DecodeSession(model, 2, context=6, max_new=4, prefix=mine).step()  # random rows follow the session's prefix
+    assert _error() == 0
