@@ -562,13 +562,15 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, q_norm_w: torch.Ten
         _need(cache_slot, "cache_slot", torch.int32, 1)
     if cache_rows is not None:
         _need(cache_rows, "cache_rows", torch.int32, 1)
-        if cache_rows.shape[0] != qkv.shape[0]:
-            raise ValueError("cache_rows must hold one row per token")
+        if cache_rows.shape[0] != qkv.shape[0] or cache_rows.device != qkv.device:
+            raise ValueError("cache_rows must hold one row per token, on the tokens' device")
     if (row_tokens is None) != (row_weights is None):
         raise ValueError("row_tokens and row_weights go together")
     if row_tokens is not None:
         _need_rows(row_tokens, "row_tokens", torch.int32, k_cache)
         _need_rows(row_weights, "row_weights", torch.float32, k_cache)
+        if nkv != k_cache.shape[1] or v_cache.shape != k_cache.shape:
+            raise ValueError(f"the caches must have {nkv} KV heads like the tokens")
     T = qkv.shape[0]
     hd = k_cache.shape[3]
     dev = qkv.device

@@ -214,3 +214,21 @@ def test_a_session_steps_behind_the_prefix_of_its_caches(cuda_dev):
         sess.step()
         DecodeSession(model, 2, context=6, max_new=4, prefix=mine).step()  # random rows follow the session's prefix
     assert _error() == 0
+
+
+def test_append_refuses_rows_of_other_heads(cuda_dev):
+    """Totals and tokens of a cache with fewer KV heads than the tokens have
+    would be written past their end."""
+    from nki_moe_7013_b200 import ops
+
+    g = _gen(16)
+    nh, nkv, T = 8, 4, 3
+    qkv, ones, freq = _randn(g, T, (nh + 2 * nkv) * HD), torch.ones(HD, device="cuda"), torch.ones(64, device="cuda")
+    for heads, v_heads in ((2, 2), (4, 2)):
+        k, v = _randn(g, 1, heads, 8, HD), _randn(g, 1, v_heads, 8, HD)
+        tok, w = torch.zeros(1, heads, 8, dtype=torch.int32, device="cuda"), torch.zeros(1, heads, 8, device="cuda")
+        with pytest.raises(ValueError, match="KV heads"):
+            ops.qk_norm_rope(qkv, _i32([0, 1, 2]), ones, ones, freq, nh, nkv, 1e-6, k, v, row_tokens=tok, row_weights=w)
+    with pytest.raises(ValueError, match="one row per token"):
+        ops.qk_norm_rope(qkv, _i32([0, 1, 2]), ones, ones, freq, nh, nkv, 1e-6, k, k, cache_rows=_i32([0, 1]))
+    assert _error() == 0
