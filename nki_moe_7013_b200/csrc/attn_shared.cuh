@@ -16,14 +16,23 @@
 // / sum_i 2^(m_i - M) l_i.  The joined M and l also turn the scores of the
 // own rows, kept in fp32 by the first kernel, into attention weights.  Own
 // rows are cut by the batch's total, so that every part of a ragged batch holds
-// about as many rows.  Short calls run as one CTA per (sequence, KV head) over
-// prefix and own rows, without a second kernel (5.2 us instead of 6.7 for two
-// sequences of 5 rows behind 129).
+// about as many rows -- while the sequences are too few to fill the SMs; more of
+// them are one part each, however uneven.  Short calls run as one CTA per
+// (sequence, KV head) over prefix and own rows, without a second kernel (5.2 us
+// instead of 6.7 for two sequences of 5 rows behind 129).
 //
 // Bound by HBM: 8 sequences of 1,400 to 4,096 rows (45 MB) stream at the copy
 // rate once the pipeline runs; 3.5 us before it (lengths, the cut, the first
 // tile's latency), 1.3 us of merging the warps and the joining kernel remain on
 // top: 21 us a call with weights, against 7 us of bytes.
+//
+// Scores, running maxima, sums and outputs are fp32.  Probabilities enter the
+// second product as bf16, the type that its other operand, V, has on the tensor
+// core; their sum l is taken before that rounding (at most 2^-8 of each, of
+// either sign, so most of it averages out over the keys).  exp2 is the
+// approximate instruction where a key costs one; the joins use exp2f.  Against
+// 64 bits the outputs are off by 0.0017 to 0.0021 of their norm, of which their
+// own rounding to bf16 is 0.0017.
 #pragma once
 
 #include "attention.cuh"
@@ -138,10 +147,9 @@ __device__ __forceinline__ bool slot_seen_before(const int32_t* cache_slot, int 
   return __any_sync(0xFFFFFFFFu, hit);
 }
 
-// One lane of a converged warp, chosen so that the compiler knows it is one: a
-// role that issues MMAs under it keeps their descriptors in uniform registers.
-// (Under lane == 0 every tcgen05.mma is wrapped in a loop over the lanes and
-// takes 120 cycles to issue, whatever its size; under this one 16.)
+// One lane of a converged warp, for a role that issues MMAs: measured, a
+// tcgen05.mma takes 16 cycles to issue under it, and 120, whatever its size,
+// under lane == 0.
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile(
@@ -412,7 +420,7 @@ __global__ void __launch_bounds__(kSdThreads)
             for (int e = 0; e < 2; ++e) s[nt][2 * h + e] = fa_exp2(s[nt][2 * h + e] - base);
           l[h] += (s[0][2 * h] + s[0][2 * h + 1]) + (s[1][2 * h] + s[1][2 * h + 1]);
         }
-        // P in bf16 (in [0, 2^8], relative rounding 2^-8): the tensor core's operand type
+        // P in bf16 (in [0, 2^8], relative rounding 2^-8), as the tensor core takes it beside a bf16 V
         uint32_t pa[4];
         pa[0] = pack_bf16x2(s[0][0], s[0][1]);
         pa[1] = pack_bf16x2(s[0][2], s[0][3]);

@@ -21,8 +21,9 @@
 // Four K tiles per query tile: a quarter of the query tiles' traffic through L2
 // (550 MB with one, for a 4,096-token prompt: 124 us instead of 111).  Then the
 // exponentials bound it: 128 x 128 per tile at 16 a cycle and SM are 1,024
-// cycles, against 512 of the products; measured 1,250 a tile, in 111 us for a
-// 4,096-token prompt (0.62 PFLOP/s).  (A quarter or a half of the exponentials
+// cycles, against 512 of the products; measured some 1,230 a tile, in 109 us for
+// a 4,096-token prompt (0.63 PFLOP/s).  (The approximate exp2 leaves the totals
+// within 1e-7 to 6e-7 of 64 bits.)  (A quarter or a half of the exponentials
 // as a degree-5 polynomial on the FMA pipe changed nothing or cost 5 %: ten
 // multiply-adds take as long as they save.  Three K tiles with a fourth
 // accumulator to fill ahead took 142 us.)

@@ -25,13 +25,16 @@
 // (each thread reads both groups' O of its TMEM lane): half the steps, for twice
 // the CTAs, where the row tiles are too few to fill the SMs, or half the parts
 // of a decode step.  S and O stay in TMEM (512 columns); P goes to
-// shared memory in bf16.  A row's O is rescaled only when its maximum grew by
+// shared memory in bf16, as the tensor core takes it beside a bf16 V (half a
+// step, 2^-8 of each probability; their sum is taken before, in fp32).  A row's
+// O is rescaled only when its maximum grew by
 // more than 2^8.
 //
 // Bound by the softmax beside the tensor core: 4 sequences of 2,048 queries
-// behind 4,096 rows take 0.61 to 0.64 ms (1.08 to 1.13 PFLOP/s, 0.65 to 0.68 of
-// the measured bf16 burst and 0.77 to 0.81 of the sustained rate; the card is at
-// its power limit), 0.52 ms without the exponentials, 0.61 without the second
+// behind 4,096 rows take 0.64 ms when repeated (1.07 PFLOP/s, 0.64 of the
+// measured bf16 burst and 0.77 of the sustained rate; the card is at its power
+// limit, at 1,732 MHz), 0.61 to 0.63 in short bursts and up to 0.69 after other
+// work; in bursts 0.52 ms without the exponentials, 0.61 without the second
 // product.  The head-packed row tiles took 8 short prompts of 37 queries behind
 // 1,001 rows from 53 to 17 us.
 //

@@ -20,7 +20,7 @@
 // newest token, two to four digits, ranks, the lists) of some 1,500 to 5,000
 // cycles each, a barrier of the CTA or its cluster after every one, and the
 // move waits for it.  8 sequences of 2,176 rows to 2,048 take 15.9 us, 4 of
-// up to 16,384 to 2,048 (28 MB moved) 23.6.
+// up to 16,384 to 2,048 (28 MB moved) 23.7.
 #pragma once
 
 #include "attn_shared.cuh"

@@ -202,8 +202,9 @@ constexpr int kQkMaxHeadsPerWarp = 16;  // nh + 2 * nkv <= 128
 
 // kRows: the cache row may differ from the position (a cache behind a prefix,
 // or one that evicts), and the row's token and weight entries may be set.  A
-// form of its own: as a run-time choice it took 7 % more at 16,384 tokens (111
-// and 118 us).
+// form of its own: as a run-time choice the plain append took 5 % more at 16,384
+// tokens (118 us for 112).  This form takes 115 there, against 52 us of bytes,
+// and 2.7 for 32 tokens.
 template <bool kRows>
 __global__ void __launch_bounds__(256)
     qk_norm_rope_kernel(const __nv_bfloat16* __restrict__ qkv, const int32_t* __restrict__ positions,

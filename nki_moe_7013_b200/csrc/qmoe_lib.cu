@@ -979,7 +979,8 @@ struct SharedDecodePlan {
 };
 
 // Rows (prefix and own) up to which a sequence's keys are not cut: 512, and
-// 1,024 where the CTAs are 32 or more.  Measured, cut and uncut: 300 rows of 8
+// 1,024 where the CTAs are 32 or more.  Measured up to 32 sequences (more were
+// not, nor against the tcgen05 prefix part), cut and uncut: 300 rows of 8
 // sequences 12.1 and 5.9 us, 500 rows of one sequence 7.9 and 7.8, 800 rows of
 // one 8.1 and 10.5, of 8 13.4 and 10.7, of 32 17.2 and 11.8.
 constexpr int64_t kDirectRows = 512;
@@ -1047,7 +1048,8 @@ SharedDecodePlan shared_decode_plan(int64_t B, int64_t G, int64_t nkv, int64_t P
     // most of the time (32 sequences of up to 700 rows on 2,048: two 20.7 us, one
     // 18.6; 16 of 4,000 on 2,048 30.9 and 26.5; without a prefix 4 of 4,096 14.1
     // and 15.4); every sequence has a part of its own, none shorter than 128 rows
-    // but its last.  Sequences that fill the SMs so are not cut.
+    // but its last.  Sequences that fill the SMs so are not cut, even where one is
+    // much longer than the others and keeps its CTAs busy alone.
     const int64_t fill = p.tc ? sms : 2 * sms;
     // Each sequence's last part is short, about half a one a sequence too many:
     // alone on the SMs that would be a second wave, so fewer are aimed at (32
