@@ -31,7 +31,7 @@
 // core; their sum l is taken before that rounding (at most 2^-8 of each, of
 // either sign, so most of it averages out over the keys).  exp2 is the
 // approximate instruction where a key costs one; the joins use exp2f.  Against
-// 64 bits the outputs are off by 0.0017 to 0.0021 of their norm, of which their
+// 64 bits the outputs are off by 0.0017 to 0.0022 of their norm, of which their
 // own rounding to bf16 is 0.0017.
 #pragma once
 
